@@ -223,6 +223,58 @@ int h3a_attn_fwd_blocksparse_tiles_ws(const void *q, const void *k, const void *
                                       h3a_stream_t stream);
 
 /*
+ * Attention over a sliding window with a few first keys that stay visible.
+ * q, o: [B,H,Sq,D], k, v: [B,Hkv,Skv,D], bf16, D == 128; Hkv divides H, and
+ * heads h*H/Hkv .. (h+1)*H/Hkv - 1 share key head h.  Row i of sequence b sits at
+ * position pos = start + i and sees key j iff
+ *   j < len  and  (pos - left <= j <= pos + right or j < sinks)
+ *   and, if causal, j <= pos
+ * where start = q_starts[b] (or q_start) and len = kv_lens[b], clamped to
+ * [0, Skv] (or Skv).  A row at a position outside [0, len) belongs to no token:
+ * its O is 0 and its lse -inf, whatever its q holds; keys at or past len are not read.
+ * A key hidden from a row contributes nothing to it, whatever it holds.
+ */
+typedef struct {
+  int left, right;          /* keys seen to either side of a position, >= 0 */
+  int sinks;                /* first keys seen from every position, >= 0 */
+  int causal;               /* no key past the position (right and sinks included) */
+  int q_start;              /* position of row 0; 0 <= q_start <= Skv - Sq unless q_starts is given */
+  const int32_t *q_starts;  /* [B] on the device, or NULL */
+  const int32_t *kv_lens;   /* [B] on the device, or NULL: Skv keys */
+} h3a_window;
+
+/*
+ * Forward.  lse [B,H,Sq] fp32 contiguous (may be NULL): log of the sum of
+ * exp(scale * q.k) over the keys seen, for h3a_attn_bwd_window.  Strides and
+ * alignment as h3a_attn_fwd, and every sequence stride < 2^24 elements; lengths
+ * up to 2^29.  No counterpart in the reference.
+ */
+int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, float *lse,
+                        int B, int H, int Hkv, int Sq, int Skv, int D,
+                        const int64_t q_strides[3], const int64_t k_strides[3],
+                        const int64_t v_strides[3], const int64_t o_strides[3],
+                        const h3a_window *window, float scale, h3a_stream_t stream);
+
+/*
+ * Backward: dq, dk, dv (bf16, in the shapes of q, k, v) from dout (bf16, as o) and
+ * the forward's o and lse; dk and dv are sums over the heads that share a key
+ * head.  Rows that belong to no token get dq = 0 and give no gradient, keys at or
+ * past len get dk = dv = 0.  The sums run in a fixed order: equal calls give equal
+ * bits.  workspace: h3a_attn_bwd_window_workspace_size bytes, untouched until the
+ * call's work has completed.
+ */
+int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, size_t *bytes);
+int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const void *v, const void *o,
+                        const float *lse, void *dq, void *dk, void *dv,
+                        int B, int H, int Hkv, int Sq, int Skv, int D,
+                        const int64_t dout_strides[3], const int64_t q_strides[3],
+                        const int64_t k_strides[3], const int64_t v_strides[3],
+                        const int64_t o_strides[3], const int64_t dq_strides[3],
+                        const int64_t dk_strides[3], const int64_t dv_strides[3],
+                        const h3a_window *window, float scale, void *workspace, size_t workspace_bytes,
+                        h3a_stream_t stream);
+
+/*
  * Convert a 0/1 block map [B,H,ceil(Sq/blk_q),ceil(Skv/blk_k)] (uint8,
  * contiguous) at any block sizes that are multiples of 16 into the tile LUT of
  * h3a_attn_fwd_blocksparse_tiles: tile_lut [B,H,ceil(Sq/64),max_tiles] (-1

@@ -138,6 +138,70 @@ void fill_attn_args(AttnArgs &a, const void *q, const void *k, const void *v, vo
   a.split_first = INT_MAX; a.split_pieces = 1; a.tile_rows = 256; a.ws = nullptr; a.sched = nullptr; a.pair_map = nullptr;
 }
 
+// Checks shared by the windowed attention entry points.
+constexpr int kMaxWindowLen = 1 << 29;
+int check_window_sizes(int B, int H, int Hkv, int Sq, int Skv, int D) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0)
+    return fail(H3A_ERR_INVALID_ARG, "sizes must be positive (B=%d H=%d Hkv=%d Sq=%d Skv=%d)", B, H, Hkv, Sq, Skv);
+  if (D != 128) return fail(H3A_ERR_UNSUPPORTED, "head_dim %d unsupported (only 128)", D);
+  if (H % Hkv != 0) return fail(H3A_ERR_INVALID_ARG, "%d key heads do not divide %d heads", Hkv, H);
+  if (Sq > kMaxWindowLen || Skv > kMaxWindowLen) return fail(H3A_ERR_INVALID_ARG, "sequence too long");
+  // Workgroups of the largest launch, one per 128 rows of a head.
+  const int64_t longest = Sq > Skv ? Sq : Skv;
+  if ((int64_t)B * H * ((longest + 127) / 128) > INT_MAX) return fail(H3A_ERR_UNSUPPORTED, "too many query or key tiles");
+  return H3A_OK;
+}
+
+int check_window(const h3a_window *w, int Sq, int Skv, float scale) {
+  if (!w) return fail(H3A_ERR_INVALID_ARG, "null window");
+  if (w->left < 0 || w->right < 0 || w->sinks < 0)
+    return fail(H3A_ERR_INVALID_ARG, "window sides and sinks must not be negative (left=%d right=%d sinks=%d)", w->left,
+                w->right, w->sinks);
+  if (!w->q_starts && (w->q_start < 0 || w->q_start > Skv - Sq))
+    return fail(H3A_ERR_INVALID_ARG, "q_start %d: rows must lie at positions 0 .. Skv - 1 (Sq=%d Skv=%d)", w->q_start,
+                Sq, Skv);
+  if ((reinterpret_cast<uintptr_t>(w->q_starts) | reinterpret_cast<uintptr_t>(w->kv_lens)) & 3u)
+    return fail(H3A_ERR_ALIGNMENT, "q_starts and kv_lens must be 4-byte aligned");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return fail(H3A_ERR_INVALID_ARG, "softmax scale must be finite and > 0");
+  return H3A_OK;
+}
+
+// One tensor of S rows: pointer, strides; written ones must not overlap themselves.
+int check_rows(const char *name, const void *p, const int64_t *st, int S, bool written) {
+  if (!p || !st) return fail(H3A_ERR_INVALID_ARG, "%s: null pointer or strides", name);
+  if (!aligned16(p)) return fail(H3A_ERR_ALIGNMENT, "%s must be 16-byte aligned", name);
+  if (!strides_ok(st)) return fail(H3A_ERR_ALIGNMENT, "%s strides must be non-negative multiples of 8 elements", name);
+  if (S > 1 && st[2] >= kMaxSeqStride)
+    return fail(H3A_ERR_UNSUPPORTED, "%s sequence stride must be < %lld elements", name, (long long)kMaxSeqStride);
+  if (written && S > 1 && st[2] < kRowElems)
+    return fail(H3A_ERR_INVALID_ARG, "%s sequence stride %lld is less than a row (%lld elements): rows overlap", name,
+                (long long)st[2], (long long)kRowElems);
+  return H3A_OK;
+}
+
+// Strides for the kernels: a length-1 sequence's is free and never reaches a row.
+void put_strides(int64_t &b, int64_t &h, int64_t &s, const int64_t *st, int S) {
+  b = st[0];
+  h = st[1];
+  s = S == 1 ? kRowElems : st[2];
+}
+
+void fill_window_args(WindowArgs &a, int B, int H, int Hkv, int Sq, int Skv, const h3a_window &w, float scale) {
+  a = WindowArgs{};
+  a.B = B; a.H = H; a.Hkv = Hkv; a.rep = H / Hkv; a.Sq = Sq; a.Skv = Skv;
+  // A side of Skv keys or more is no limit; clamped, positions plus sides fit an int.
+  a.left = w.left < Skv ? w.left : Skv;
+  a.right = w.causal ? 0 : (w.right < Skv ? w.right : Skv);
+  a.sinks = w.sinks < Skv ? w.sinks : Skv;
+  a.causal = w.causal != 0;
+  a.q_start = w.q_start; a.q_starts = w.q_starts; a.kv_lens = w.kv_lens;
+  a.scale = scale;
+  a.sl2 = scale * 1.4426950408889634f;
+}
+
+size_t window_bwd_bytes(int B, int H, int Sq) { return (size_t)B * H * Sq * sizeof(float); }
+
 }  // namespace
 }  // namespace h3a
 
@@ -404,6 +468,90 @@ int h3a_attn_fwd_blocksparse_tiles_ws(const void *q, const void *k, const void *
     if (!aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
   }
   return launch_attn_sparse_split(a, 64, plan, workspace, as_stream(stream), true);
+}
+
+int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, float *lse, int B, int H, int Hkv,
+                        int Sq, int Skv, int D, const int64_t q_strides[3], const int64_t k_strides[3],
+                        const int64_t v_strides[3], const int64_t o_strides[3], const h3a_window *window,
+                        float scale, h3a_stream_t stream) {
+  clear_error();
+  int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
+  if (!rc) rc = check_window(window, Sq, Skv, scale);
+  if (!rc) rc = check_rows("q", q, q_strides, Sq, false);
+  if (!rc) rc = check_rows("k", k, k_strides, Skv, false);
+  if (!rc) rc = check_rows("v", v, v_strides, Skv, false);
+  if (!rc) rc = check_rows("o", o, o_strides, Sq, true);
+  if (rc) return rc;
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(H3A_ERR_ALIGNMENT, "lse must be 4-byte aligned");
+  WindowArgs a;
+  fill_window_args(a, B, H, Hkv, Sq, Skv, *window, scale);
+  a.q = static_cast<const uint16_t *>(q);
+  a.k = static_cast<const uint16_t *>(k);
+  a.v = static_cast<const uint16_t *>(v);
+  a.o = static_cast<uint16_t *>(o);
+  a.lse = lse;
+  put_strides(a.qsb, a.qsh, a.qss, q_strides, Sq);
+  put_strides(a.ksb, a.ksh, a.kss, k_strides, Skv);
+  put_strides(a.vsb, a.vsh, a.vss, v_strides, Skv);
+  put_strides(a.osb, a.osh, a.oss, o_strides, Sq);
+  return launch_window_fwd(a, as_stream(stream));
+}
+
+int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, size_t *bytes) {
+  clear_error();
+  if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
+  const int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
+  if (rc) return rc;
+  *bytes = window_bwd_bytes(B, H, Sq);
+  return H3A_OK;
+}
+
+int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const void *v, const void *o,
+                        const float *lse, void *dq, void *dk, void *dv, int B, int H, int Hkv, int Sq, int Skv,
+                        int D, const int64_t dout_strides[3], const int64_t q_strides[3],
+                        const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
+                        const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
+                        const h3a_window *window, float scale, void *workspace, size_t workspace_bytes,
+                        h3a_stream_t stream) {
+  clear_error();
+  int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
+  if (!rc) rc = check_window(window, Sq, Skv, scale);
+  if (!rc) rc = check_rows("dout", dout, dout_strides, Sq, false);
+  if (!rc) rc = check_rows("q", q, q_strides, Sq, false);
+  if (!rc) rc = check_rows("k", k, k_strides, Skv, false);
+  if (!rc) rc = check_rows("v", v, v_strides, Skv, false);
+  if (!rc) rc = check_rows("o", o, o_strides, Sq, false);
+  if (!rc) rc = check_rows("dq", dq, dq_strides, Sq, true);
+  if (!rc) rc = check_rows("dk", dk, dk_strides, Skv, true);
+  if (!rc) rc = check_rows("dv", dv, dv_strides, Skv, true);
+  if (rc) return rc;
+  if (!lse) return fail(H3A_ERR_INVALID_ARG, "null lse");
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(H3A_ERR_ALIGNMENT, "lse must be 4-byte aligned");
+  const size_t need = window_bwd_bytes(B, H, Sq);
+  if (!workspace || workspace_bytes < need)
+    return fail(H3A_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+  if (!aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  WindowArgs a;
+  fill_window_args(a, B, H, Hkv, Sq, Skv, *window, scale);
+  a.q = static_cast<const uint16_t *>(q);
+  a.k = static_cast<const uint16_t *>(k);
+  a.v = static_cast<const uint16_t *>(v);
+  a.o = static_cast<uint16_t *>(const_cast<void *>(o));
+  a.lse = const_cast<float *>(lse);
+  a.dout = static_cast<const uint16_t *>(dout);
+  a.dq = static_cast<uint16_t *>(dq);
+  a.dk = static_cast<uint16_t *>(dk);
+  a.dv = static_cast<uint16_t *>(dv);
+  a.delta = static_cast<float *>(workspace);
+  put_strides(a.gsb, a.gsh, a.gss, dout_strides, Sq);
+  put_strides(a.qsb, a.qsh, a.qss, q_strides, Sq);
+  put_strides(a.ksb, a.ksh, a.kss, k_strides, Skv);
+  put_strides(a.vsb, a.vsh, a.vss, v_strides, Skv);
+  put_strides(a.osb, a.osh, a.oss, o_strides, Sq);
+  put_strides(a.dqsb, a.dqsh, a.dqss, dq_strides, Sq);
+  put_strides(a.dksb, a.dksh, a.dkss, dk_strides, Skv);
+  put_strides(a.dvsb, a.dvsh, a.dvss, dv_strides, Skv);
+  return launch_window_bwd(a, as_stream(stream));
 }
 
 int h3a_block_map_to_tile_lut(const uint8_t *block_map, int B, int H, int Sq, int Skv, int blk_q, int blk_k,

@@ -118,6 +118,34 @@ int attn_kernel_attrs(int which, double out[6]);
 int attn_prof_read(uint64_t *out);  // H3A_PROF_WAVES x H3A_PROF_SLOTS
 int attn_prof_reset();
 
+// Kernel-side argument block of the windowed attention kernels (h3a_window.hip).
+struct WindowArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t *o;  // forward: written; backward: read
+  float *lse;   // [B,H,Sq], natural logarithm; forward: written unless null
+  int64_t qsb, qsh, qss;
+  int64_t ksb, ksh, kss;
+  int64_t vsb, vsh, vss;
+  int64_t osb, osh, oss;
+  int B, H, Hkv, rep, Sq, Skv;  // rep = H / Hkv heads share a key head
+  int left, right, sinks, causal;
+  int q_start;
+  const int32_t *q_starts, *kv_lens;  // per sequence, or null
+  float scale, sl2;                   // softmax scale, and times log2(e)
+  int nqt, nkt;  // 128-row query and key tiles per head
+  int total;     // workgroups
+  // backward only
+  const uint16_t *dout;
+  uint16_t *dq, *dk, *dv;
+  int64_t gsb, gsh, gss;
+  int64_t dqsb, dqsh, dqss;
+  int64_t dksb, dksh, dkss;
+  int64_t dvsb, dvsh, dvss;
+  float *delta;  // [B,H,Sq] dO.O
+};
+int launch_window_fwd(WindowArgs a, hipStream_t s);
+int launch_window_bwd(WindowArgs a, hipStream_t s);
+
 struct RopeArgs {
   uint16_t *q, *k;
   int64_t qsb, qss, qsh;

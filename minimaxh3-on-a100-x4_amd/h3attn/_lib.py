@@ -37,6 +37,13 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
 
+
+class Window(ctypes.Structure):
+    """h3a_window."""
+    _fields_ = [("left", _i), ("right", _i), ("sinks", _i), ("causal", _i), ("q_start", _i), ("q_starts", _vp),
+                ("kv_lens", _vp)]
+
+
 # Every symbol of include/h3attn.h with its (restype, argtypes).
 SIGNATURES = {
     "h3a_version": (ctypes.c_char_p, []),
@@ -63,6 +70,10 @@ SIGNATURES = {
     "h3a_attn_fwd_blocksparse_tiles_ws": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                                                _c_i64_3, _c_i64_3, _c_i64_3, _c_i64_3, _vp, _vp, _i, _f,
                                                _vp, ctypes.c_size_t, _vp]),
+    "h3a_attn_fwd_window": (_i, [_vp] * 5 + [_i] * 6 + [_c_i64_3] * 4 + [ctypes.POINTER(Window), _f, _vp]),
+    "h3a_attn_bwd_window_workspace_size": (_i, [_i] * 6 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "h3a_attn_bwd_window": (_i, [_vp] * 9 + [_i] * 6 + [_c_i64_3] * 8 + [ctypes.POINTER(Window), _f, _vp,
+                                                                         ctypes.c_size_t, _vp]),
     "h3a_block_map_to_tile_lut": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp]),
     "h3a_lut_to_block_map": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "h3a_block_map_to_lut": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _i, _vp]),

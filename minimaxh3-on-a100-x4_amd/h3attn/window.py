@@ -1,0 +1,153 @@
+"""Attention over a sliding window with a few first keys that stay visible, forward and backward.
+
+For windowed layers of the DiT, whose text tokens come first in the packed sequence
+and are seen by every video token, and for the single new token of a causal model
+against its cache of keys.  The gradients are those of the same mask; h3attn.autograd
+wraps both in a differentiable function.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import check, lib, strides3
+from .ops import HEAD_DIM, _as_kernel_input, _layout, _on_device, _stream
+
+
+def _side(name: str, n) -> int:
+    """A window side as an int; None is no limit."""
+    if n is None:
+        return 2 ** 31 - 1
+    if int(n) != n or n < 0:
+        raise ValueError(f"{name} must be a whole number >= 0 (or None for no limit), got {n}")
+    return min(int(n), 2 ** 31 - 1)
+
+
+def _per_sequence(name: str, t: torch.Tensor, B: int, device) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != B or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor [{B}] on q's device, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device) -> _lib.Window:
+    try:
+        left, right = window
+    except TypeError:
+        raise ValueError(f"window must be a pair (left, right), got {window!r}") from None
+    left, right = _side("window's left side", left), _side("window's right side", right)
+    if causal and window[1] not in (0, None):
+        raise ValueError(f"a causal window has no right side, got {window[1]}")
+    lens = None if kv_lens is None else _per_sequence("kv_lens", kv_lens, B, device)
+    start, starts = 0, None
+    if isinstance(q_start, torch.Tensor):
+        starts = _per_sequence("q_start", q_start, B, device)
+    elif q_start is None:
+        if lens is not None and Sq != Skv:
+            raise ValueError("kv_lens with Sq != Skv needs q_start: where the queries sit in the sequences")
+        start = Skv - Sq
+    else:
+        start = int(q_start)
+    if starts is None and not 0 <= start <= Skv - Sq:
+        raise ValueError(f"q_start {start}: rows must lie at positions 0 .. Skv - 1 (Sq={Sq}, Skv={Skv})")
+    return _lib.Window(left, right, _side("sinks", sinks), 1 if causal else 0, start, starts, lens)
+
+
+def _prepare(q, k, v):
+    q, qst = _as_kernel_input("q", q)
+    k, kst = _as_kernel_input("k", k)
+    v, vst = _as_kernel_input("v", v)
+    B, H, Sq, D = q.shape
+    Hkv, Skv = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or Hkv == 0 or H % Hkv:
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+    if 0 in (B, H, Sq, Skv):
+        raise ValueError("empty attention input")
+    if not (q.device == k.device == v.device):
+        raise ValueError("q, k, v must be on the same device")
+    return q, k, v, (B, H, Hkv, Sq, Skv, D), (qst, kst, vst)
+
+
+def _check_like(name: str, t: torch.Tensor, q: torch.Tensor):
+    if not isinstance(t, torch.Tensor) or t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
+        raise ValueError(f"{name} must be a bf16 tensor {tuple(q.shape)} on its device")
+
+
+def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, sinks: int = 0, causal: bool = False,
+                    scale: float | None = None, out: torch.Tensor | None = None, q_start=None,
+                    kv_lens: torch.Tensor | None = None, return_lse: bool = False):
+    """Windowed attention, q [B,H,Sq,128], k/v [B,Hkv,Skv,128] bf16 (Hkv divides H) -> O [B,H,Sq,128].
+
+    window: (left, right) keys seen to either side of a query's position, None for
+    no limit; sinks: first keys seen from every position; causal: no key past the
+    position (the window's right side is then 0 or None).
+    q_start: position of the first query row, an int or an int32 GPU tensor [B];
+    the default is Skv - Sq (the queries are the last rows), or 0 where Sq == Skv.
+    kv_lens: int32 GPU tensor [B], the sequences' lengths in a padded batch or a
+    cache; with Sq != Skv it needs q_start (kv_lens - 1 for one new token).  Rows
+    at positions outside [0, kv_lens) give O = 0 and lse = -inf.
+    return_lse: also the log-sum-exp of the scaled scores, fp32 [B,H,Sq], which
+    attn_bwd_window takes.  Strides and `out` as for attn_fwd.
+    """
+    q, k, v, (B, H, Hkv, Sq, Skv, D), st = _prepare(q, k, v)
+    w = _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, q.device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        ost = out.stride()[:3]
+    else:
+        _check_like("out", out, q)
+        ost = _layout(out)
+        if ost is None:
+            raise ValueError("out must have unit last stride, 16-byte alignment and strides multiple of 8")
+    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device) if return_lse else None
+    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    with _on_device(q):
+        rc = lib().h3a_attn_fwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                       None if lse is None else lse.data_ptr(), B, H, Hkv, Sq, Skv, D, *st,
+                                       strides3(*ost), ctypes.byref(w), sc, _stream(q))
+    check("h3a_attn_fwd_window", rc)
+    return (out, lse) if return_lse else out
+
+
+def _grad_like(t: torch.Tensor):
+    """A tensor for t's gradient, in t's order of dimensions where the kernels can write it."""
+    g = torch.empty_like(t)
+    st = _layout(g)
+    if st is None or (g.shape[2] > 1 and st[2] < HEAD_DIM):
+        g = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        st = _layout(g)
+    return g, strides3(*st)
+
+
+def attn_bwd_window(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                    lse: torch.Tensor, window, sinks: int = 0, causal: bool = False, scale: float | None = None,
+                    q_start=None, kv_lens: torch.Tensor | None = None):
+    """Gradients (dq, dk, dv) of attn_fwd_window from dout, its inputs, its O and its lse (return_lse=True).
+
+    window .. kv_lens as in the forward call.  dk and dv sum over the heads that
+    share a key head.  The sums run in a fixed order: equal calls give equal bits.
+    """
+    q, k, v, (B, H, Hkv, Sq, Skv, D), st = _prepare(q, k, v)
+    _check_like("dout", dout, q)
+    _check_like("o", o, q)
+    dout, gst = _as_kernel_input("dout", dout)
+    o, ost = _as_kernel_input("o", o)
+    if lse.shape != (B, H, Sq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError(f"lse must be the forward's fp32 [{B},{H},{Sq}] tensor")
+    w = _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, q.device)
+    (dq, dqst), (dk, dkst), (dv, dvst) = _grad_like(q), _grad_like(k), _grad_like(v)
+    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    with _on_device(q):
+        n = ctypes.c_size_t(0)
+        check("h3a_attn_bwd_window_workspace_size",
+              lib().h3a_attn_bwd_window_workspace_size(B, H, Hkv, Sq, Skv, D, ctypes.byref(n)))
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        rc = lib().h3a_attn_bwd_window(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                       lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Sq,
+                                       Skv, D, gst, *st, ost, dqst, dkst, dvst, ctypes.byref(w), sc, ws.data_ptr(),
+                                       n.value, _stream(q))
+    check("h3a_attn_bwd_window", rc)
+    return dq, dk, dv

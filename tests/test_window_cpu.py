@@ -1,0 +1,101 @@
+"""Windowed attention without a GPU: what is refused, before any HIP call."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import h3attn
+from h3attn import _lib
+
+S3 = _lib.strides3
+ROW = S3(0, 0, 128)
+
+
+def _fwd(L, q=16, k=16, v=16, o=16, lse=None, B=1, H=2, Hkv=1, Sq=4, Skv=4, D=128, st=(ROW,) * 4,
+         w=(3, 3, 1, 0, 0), starts=None, lens=None, scale=0.1):
+    win = None if w is None else ctypes.byref(_lib.Window(*w, starts, lens))
+    return L.h3a_attn_fwd_window(q, k, v, o, lse, B, H, Hkv, Sq, Skv, D, *st, win, scale, None)
+
+
+def test_forward_refusals():
+    L = _lib.lib()
+    bad, unsup, align = _lib.H3A_ERR_INVALID_ARG, _lib.H3A_ERR_UNSUPPORTED, _lib.H3A_ERR_ALIGNMENT
+    assert _fwd(L, q=None) == bad
+    assert _fwd(L, w=None) == bad
+    for size in ("B", "H", "Hkv", "Sq", "Skv"):
+        assert _fwd(L, **{size: 0}) == bad
+    assert _fwd(L, H=3, Hkv=2) == bad
+    assert _fwd(L, D=64) == unsup
+    assert _fwd(L, B=1 << 16, H=1 << 16) == unsup
+    assert _fwd(L, Skv=(1 << 29) + 1) == bad
+    for w in ((-1, 0, 0, 0, 0), (0, -1, 0, 0, 0), (0, 0, -1, 0, 0), (0, 0, 0, 0, 1), (0, 0, 0, 0, -1)):
+        assert _fwd(L, w=w) == bad
+    assert _fwd(L, Sq=5) == bad  # more rows than positions
+    assert _fwd(L, scale=0.0) == bad and _fwd(L, scale=float("inf")) == bad
+    assert _fwd(L, q=24) == align and _fwd(L, lse=18) == align and _fwd(L, lens=18) == align
+    assert _fwd(L, st=(S3(0, 0, 12), ROW, ROW, ROW)) == align
+    for i in range(4):
+        st = [ROW] * 4
+        st[i] = S3(0, 0, 1 << 24)
+        assert _fwd(L, st=tuple(st)) == unsup
+        assert b"sequence stride" in L.h3a_last_error()
+    assert _fwd(L, st=(ROW, ROW, ROW, S3(0, 0, 120))) == bad
+    assert b"rows overlap" in L.h3a_last_error()
+
+
+def test_backward_refusals():
+    L = _lib.lib()
+    n = ctypes.c_size_t(0)
+    assert L.h3a_attn_bwd_window_workspace_size(1, 2, 1, 4, 4, 128, None) == _lib.H3A_ERR_INVALID_ARG
+    assert L.h3a_attn_bwd_window_workspace_size(1, 2, 1, 4, 4, 64, ctypes.byref(n)) == _lib.H3A_ERR_UNSUPPORTED
+    assert L.h3a_attn_bwd_window_workspace_size(1, 2, 1, 4, 4, 128, ctypes.byref(n)) == 0 and n.value > 0
+
+    def bwd(ptrs=(16,) * 9, st=(ROW,) * 8, ws=16, nbytes=n.value):
+        win = _lib.Window(3, 3, 1, 0, 0, None, None)
+        return L.h3a_attn_bwd_window(*ptrs, 1, 2, 1, 4, 4, 128, *st, ctypes.byref(win), 0.1, ws, nbytes, None)
+
+    for i in range(9):
+        assert bwd(ptrs=tuple(None if i == j else 16 for j in range(9))) == _lib.H3A_ERR_INVALID_ARG
+    for i in range(8):
+        assert bwd(st=tuple(S3(0, 0, 12) if i == j else ROW for j in range(8))) == _lib.H3A_ERR_ALIGNMENT
+    for i in (5, 6, 7):
+        assert bwd(st=tuple(S3(0, 0, 64) if i == j else ROW for j in range(8))) == _lib.H3A_ERR_INVALID_ARG
+    assert bwd(ws=None) == _lib.H3A_ERR_INVALID_ARG
+    assert bwd(nbytes=n.value - 1) == _lib.H3A_ERR_INVALID_ARG
+    assert bwd(ws=24) == _lib.H3A_ERR_ALIGNMENT
+
+
+def test_python_refusals(monkeypatch):
+    from h3attn import window
+    q = torch.zeros(2, 4, 8, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        h3attn.attn_fwd_window(q, q, q, (1, 1))
+    monkeypatch.setattr(window, "_as_kernel_input", lambda name, t: (t, S3(*t.stride()[:3])))
+
+    def refused(match, q=q, k=q, v=q, window=(1, 1), **kw):
+        with pytest.raises(ValueError, match=match):
+            h3attn.attn_fwd_window(q, k, v, window, **kw)
+
+    refused("mismatch", k=q[:, :3], v=q[:, :3])
+    refused("mismatch", k=q[:1], v=q[:1])
+    refused("mismatch", v=q[:, :, :7])
+    refused("empty", q=q[:, :, :0])
+    refused("pair", window=3)
+    refused("left side", window=(-1, 0))
+    refused("right side", window=(0, 1.5))
+    refused("sinks", sinks=-2)
+    refused("causal", window=(4, 2), causal=True)
+    refused("q_start", q_start=1)
+    refused("q_start", q=q[:, :, :3], q_start=6)
+    refused("needs q_start", q=q[:, :, :3], kv_lens=torch.zeros(2, dtype=torch.int32))
+    refused("kv_lens", kv_lens=torch.zeros(2, dtype=torch.int64))
+    refused("kv_lens", kv_lens=torch.zeros(3, dtype=torch.int32))
+    refused("q_start", q_start=torch.zeros(4, dtype=torch.int32)[::2])
+    refused("out must", out=q.float())
+    lse = torch.zeros(2, 4, 8)
+    with pytest.raises(ValueError, match="dout"):
+        h3attn.attn_bwd_window(q.float(), q, q, q, q, lse, (1, 1))
+    with pytest.raises(ValueError, match="lse"):
+        h3attn.attn_bwd_window(q, q, q, q, q, lse[:, :, :7], (1, 1))
