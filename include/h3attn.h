@@ -383,6 +383,80 @@ int h3a_qk_rmsnorm_rope_pool(void *q, void *k, int B, int S, int H, int D,
                              int rot_dim, const void *qw, const void *kw, float eps,
                              int blk, float *q_means, float *k_means, h3a_stream_t stream);
 
+/*
+ * The prologue from positions on several axes (time, height, width) instead of a
+ * table: q and k may differ in heads, and the outputs may be other memory than the
+ * inputs (a training step keeps those) or the same.  q: [B,S,Hq,D], k: [B,S,Hk,D]
+ * bf16, *_strides = {batch, seq, head}; D == 128.  With rot = sum of dims, pair
+ * (i, i + rot/2), i < rot/2, belongs to the axis whose dims/2 pairs, axis after
+ * axis, hold i; as pair n of an axis of d dims it turns by
+ *   angle = pos[b,s,axis] * theta^(-2n/d)
+ * in the sense of h3a_qk_rmsnorm_rope's R = [[cos, -sin], [sin, cos]].  Angles are
+ * taken in 64 bits.  dims: even; rot a multiple of 16, <= D.  No counterpart in the
+ * reference, whose caller brings the table.
+ */
+#define H3A_MAX_AXES 4
+typedef struct {
+  const void *pos;        /* [S, axes], or [B, S, axes] with batch_stride; contiguous, on the device */
+  int64_t batch_stride;   /* elements of pos from sequence to sequence; 0: the same positions for all */
+  int pos_float;          /* 0: int32, 1: fp32 */
+  int axes;               /* 1 .. H3A_MAX_AXES */
+  int dims[H3A_MAX_AXES]; /* rotated dims of each axis */
+  double theta;
+} h3a_positions;
+int h3a_qk_rmsnorm_rope_axes(const void *q, const void *k, void *q_out, void *k_out,
+                             int B, int S, int Hq, int Hk, int D,
+                             const int64_t q_strides[3], const int64_t k_strides[3],
+                             const int64_t q_out_strides[3], const int64_t k_out_strides[3],
+                             const h3a_positions *positions, const void *qw, const void *kw, float eps,
+                             h3a_stream_t stream);
+
+/*
+ * Its backward: from the gradients of q_out and k_out (q_dout, k_dout, bf16) and the
+ * forward's inputs, the gradients of q and k (q_grad, k_grad, bf16) and of the
+ * weights (qw_grad, kw_grad [D] fp32, summed over all rows in a fixed order).
+ * workspace: h3a_qk_rmsnorm_rope_axes_bwd_workspace_size bytes.
+ */
+int h3a_qk_rmsnorm_rope_axes_bwd_workspace_size(int B, int S, size_t *bytes);
+int h3a_qk_rmsnorm_rope_axes_bwd(const void *q_dout, const void *k_dout, const void *q, const void *k,
+                                 void *q_grad, void *k_grad, float *qw_grad, float *kw_grad,
+                                 int B, int S, int Hq, int Hk, int D,
+                                 const int64_t q_dout_strides[3], const int64_t k_dout_strides[3],
+                                 const int64_t q_strides[3], const int64_t k_strides[3],
+                                 const int64_t q_grad_strides[3], const int64_t k_grad_strides[3],
+                                 const h3a_positions *positions, const void *qw, const void *kw, float eps,
+                                 void *workspace, size_t workspace_bytes, h3a_stream_t stream);
+
+/*
+ * Layer norm of x [rows, C] (channels contiguous, *_stride elements from row to row)
+ * with a scale and shift per segment of rows: rows bounds[s] .. bounds[s+1]-1 take
+ * row s of w and b [segments, C] (contiguous; either may be NULL: 1, 0):
+ *   y = (x - mean) * rstd * w + b, or (1 + w) in place of w (modulate, as the DiT's
+ *   adaLN, harness/sp_runtime.py:203-218).
+ * bounds is host memory, segments + 1 non-decreasing ints from 0 to rows; a segment
+ * may be empty.  x and y share dtype; w and b share w_dtype (H3A_BF16, H3A_FP16 or
+ * H3A_FP32).  mean, rstd [rows] fp32 (both or neither NULL) are kept for the
+ * backward.  y may be x.  rows may be 0; C <= 16384.
+ */
+#define H3A_BF16 0
+#define H3A_FP16 1
+#define H3A_FP32 2
+int h3a_layer_norm_fwd(const void *x, int64_t x_stride, const void *w, const void *b, void *y, int64_t y_stride,
+                       float *mean, float *rstd, int rows, int C, int dtype, int w_dtype, const int *bounds,
+                       int segments, int modulate, float eps, h3a_stream_t stream);
+
+/*
+ * Its backward: dx (dtype of x), and, unless both are NULL, dw and db [segments, C]
+ * fp32, the gradients of w and b, summed over each segment's rows in a fixed order
+ * (0 for an empty one).  dx may be dy or x.  workspace (only with dw and db):
+ * h3a_layer_norm_bwd_workspace_size bytes.
+ */
+int h3a_layer_norm_bwd_workspace_size(const int *bounds, int segments, int C, size_t *bytes);
+int h3a_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *w,
+                       const float *mean, const float *rstd, void *dx, int64_t dx_stride, float *dw, float *db,
+                       int rows, int C, int dtype, int w_dtype, const int *bounds, int segments, int modulate,
+                       void *workspace, size_t workspace_bytes, h3a_stream_t stream);
+
 /* Kernel identifiers for h3a_kernel_attrs. */
 #define H3A_KERNEL_ATTN_DENSE      0
 #define H3A_KERNEL_ATTN_SPARSE_128 1

@@ -200,6 +200,98 @@ void fill_window_args(WindowArgs &a, int B, int H, int Hkv, int Sq, int Skv, con
   a.sl2 = scale * 1.4426950408889634f;
 }
 
+// The prologue from positions: sizes, and the angles' steps in revolutions.
+int fill_rope_axes(RopeAxesArgs &a, int B, int S, int Hq, int Hk, int D, const h3a_positions *p, const void *qw,
+                   const void *kw, float eps) {
+  if (B <= 0 || S <= 0 || Hq <= 0 || Hk <= 0)
+    return fail(H3A_ERR_INVALID_ARG, "sizes must be positive (B=%d S=%d Hq=%d Hk=%d)", B, S, Hq, Hk);
+  if (D != 128) return fail(H3A_ERR_UNSUPPORTED, "head_dim %d unsupported (only 128)", D);
+  if (!p || !p->pos || !qw || !kw) return fail(H3A_ERR_INVALID_ARG, "null positions or weights");
+  if (p->axes < 1 || p->axes > H3A_MAX_AXES)
+    return fail(H3A_ERR_UNSUPPORTED, "%d axes unsupported (1 to %d)", p->axes, H3A_MAX_AXES);
+  if (!(p->theta > 0.0) || !std::isfinite(p->theta)) return fail(H3A_ERR_INVALID_ARG, "theta must be finite and > 0");
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(H3A_ERR_INVALID_ARG, "eps must be finite and >= 0");
+  if (p->batch_stride < 0) return fail(H3A_ERR_INVALID_ARG, "negative batch stride of the positions");
+  if (reinterpret_cast<uintptr_t>(p->pos) & 3u) return fail(H3A_ERR_ALIGNMENT, "positions must be 4-byte aligned");
+  if (!aligned16(qw) || !aligned16(kw)) return fail(H3A_ERR_ALIGNMENT, "weights must be 16-byte aligned");
+  a = RopeAxesArgs{};
+  int rot = 0;
+  for (int x = 0; x < p->axes; ++x) {
+    const int d = p->dims[x];
+    if (d <= 0 || d % 2 != 0 || d > D - rot)
+      return fail(H3A_ERR_UNSUPPORTED, "axis %d: %d dims (even numbers that add up to at most %d)", x, d, D);
+    for (int n = 0; n < d / 2; ++n) {
+      a.turns[rot / 2 + n] = std::pow(p->theta, -2.0 * n / d) / 6.283185307179586476925286766559;
+      a.axis[rot / 2 + n] = (uint8_t)x;
+    }
+    rot += d;
+  }
+  if (rot % 16 != 0) return fail(H3A_ERR_UNSUPPORTED, "rotated dims %d must be a multiple of 16", rot);
+  a.B = B; a.S = S; a.H[0] = Hq; a.H[1] = Hk;
+  a.rot = rot;
+  a.eps = eps;
+  a.pos = p->pos; a.pos_float = p->pos_float != 0; a.axes = p->axes; a.pos_b = p->batch_stride;
+  a.w[0] = static_cast<const uint16_t *>(qw);
+  a.w[1] = static_cast<const uint16_t *>(kw);
+  return H3A_OK;
+}
+
+// A [B,S,H,128] tensor of it; strides of size-1 dimensions are free.
+int put_rope_tensor(const char *name, const void *p, const int64_t *st, bool written, int B, int S, int H,
+                    int64_t (&to)[3]) {
+  if (!p || !st) return fail(H3A_ERR_INVALID_ARG, "%s: null pointer or strides", name);
+  if (!aligned16(p)) return fail(H3A_ERR_ALIGNMENT, "%s must be 16-byte aligned", name);
+  if (!strides_ok(st)) return fail(H3A_ERR_ALIGNMENT, "%s strides must be non-negative multiples of 8 elements", name);
+  const int n[3] = {B, S, H};
+  for (int i = 0; i < 3; ++i) {
+    to[i] = n[i] == 1 ? 0 : st[i];
+    if (written && n[i] > 1 && st[i] < kRowElems)
+      return fail(H3A_ERR_INVALID_ARG, "%s stride %lld is less than a row (%lld elements): rows overlap", name,
+                  (long long)st[i], (long long)kRowElems);
+  }
+  return H3A_OK;
+}
+
+size_t rope_axes_bwd_bytes(int B, int S) { return (size_t)rope_axes_bwd_wgs(B, S) * 256 * sizeof(float); }
+
+// Layer norm: sizes, types and segments.
+int check_norm(int rows, int C, int dtype, int w_dtype, const int *bounds, int segments) {
+  if (rows < 0 || C <= 0) return fail(H3A_ERR_INVALID_ARG, "bad sizes (rows=%d C=%d)", rows, C);
+  if (C > 16384) return fail(H3A_ERR_UNSUPPORTED, "%d channels unsupported (at most 16384)", C);
+  for (int d : {dtype, w_dtype})
+    if (d != H3A_BF16 && d != H3A_FP16 && d != H3A_FP32) return fail(H3A_ERR_UNSUPPORTED, "dtype %d unsupported", d);
+  if (!bounds || segments <= 0) return fail(H3A_ERR_INVALID_ARG, "no segments");
+  if (bounds[0] != 0 || bounds[segments] != rows)
+    return fail(H3A_ERR_INVALID_ARG, "bounds must run from 0 to %d rows (%d .. %d)", rows, bounds[0], bounds[segments]);
+  for (int s = 0; s < segments; ++s)
+    if (bounds[s + 1] < bounds[s]) return fail(H3A_ERR_INVALID_ARG, "bounds decrease at segment %d", s);
+  return H3A_OK;
+}
+
+int norm_rows(const char *name, const void *p, int64_t stride, int rows, int C, int dtype, bool written, bool *vec,
+              int64_t *bytes) {
+  if (rows == 0) return H3A_OK;
+  if (!p) return fail(H3A_ERR_INVALID_ARG, "%s: null pointer", name);
+  const int size = dtype == H3A_FP32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(p) % size) return fail(H3A_ERR_ALIGNMENT, "%s is not aligned to its elements", name);
+  if (rows > 1 && (stride < 0 || (written && stride < C)))
+    return fail(H3A_ERR_INVALID_ARG, "%s row stride %lld: rows overlap", name, (long long)stride);
+  *bytes = rows == 1 ? 0 : stride * size;
+  if (!aligned16(p) || *bytes % 16 != 0) *vec = false;
+  return H3A_OK;
+}
+
+int norm_affine(const char *name, const void *p, int w_dtype) {
+  if (reinterpret_cast<uintptr_t>(p) % (w_dtype == H3A_FP32 ? 4 : 2))
+    return fail(H3A_ERR_ALIGNMENT, "%s is not aligned to its elements", name);
+  return H3A_OK;
+}
+
+size_t norm_bwd_bytes(const int *bounds, int segments, int C) {
+  const int wgs = norm_wgs(bounds, segments, norm_rows_per_wg(bounds[segments], C, kNormBwdWgs));
+  return (size_t)wgs * 2 * C * sizeof(float);
+}
+
 size_t window_bwd_bytes(int B, int H, int Sq) { return (size_t)B * H * Sq * sizeof(float); }
 
 }  // namespace
@@ -706,6 +798,139 @@ int h3a_qk_rmsnorm_rope_pool(void *q, void *k, int B, int S, int H, int D, const
   const int64_t wgs = (int64_t)B * ((S + blk - 1) / blk) * ((H + 7) / 8);
   if (wgs > INT_MAX) return fail(H3A_ERR_INVALID_ARG, "too many blocks");
   return launch_qk_rmsnorm_rope_pool(a, blk, q_means, k_means, as_stream(stream));
+}
+
+int h3a_qk_rmsnorm_rope_axes(const void *q, const void *k, void *q_out, void *k_out, int B, int S, int Hq, int Hk,
+                             int D, const int64_t q_strides[3], const int64_t k_strides[3],
+                             const int64_t q_out_strides[3], const int64_t k_out_strides[3],
+                             const h3a_positions *positions, const void *qw, const void *kw, float eps,
+                             h3a_stream_t stream) {
+  clear_error();
+  RopeAxesArgs a;
+  int rc = fill_rope_axes(a, B, S, Hq, Hk, D, positions, qw, kw, eps);
+  if (!rc) rc = put_rope_tensor("q", q, q_strides, false, B, S, Hq, a.xs[0]);
+  if (!rc) rc = put_rope_tensor("k", k, k_strides, false, B, S, Hk, a.xs[1]);
+  if (!rc) rc = put_rope_tensor("q_out", q_out, q_out_strides, true, B, S, Hq, a.ys[0]);
+  if (!rc) rc = put_rope_tensor("k_out", k_out, k_out_strides, true, B, S, Hk, a.ys[1]);
+  if (rc) return rc;
+  a.x[0] = static_cast<const uint16_t *>(q);
+  a.x[1] = static_cast<const uint16_t *>(k);
+  a.y[0] = static_cast<uint16_t *>(q_out);
+  a.y[1] = static_cast<uint16_t *>(k_out);
+  return launch_rope_axes(a, false, as_stream(stream));
+}
+
+int h3a_qk_rmsnorm_rope_axes_bwd_workspace_size(int B, int S, size_t *bytes) {
+  clear_error();
+  if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
+  if (B <= 0 || S <= 0) return fail(H3A_ERR_INVALID_ARG, "sizes must be positive (B=%d S=%d)", B, S);
+  *bytes = rope_axes_bwd_bytes(B, S);
+  return H3A_OK;
+}
+
+int h3a_qk_rmsnorm_rope_axes_bwd(const void *q_dout, const void *k_dout, const void *q, const void *k, void *q_grad,
+                                 void *k_grad, float *qw_grad, float *kw_grad, int B, int S, int Hq, int Hk, int D,
+                                 const int64_t q_dout_strides[3], const int64_t k_dout_strides[3],
+                                 const int64_t q_strides[3], const int64_t k_strides[3],
+                                 const int64_t q_grad_strides[3], const int64_t k_grad_strides[3],
+                                 const h3a_positions *positions, const void *qw, const void *kw, float eps,
+                                 void *workspace, size_t workspace_bytes, h3a_stream_t stream) {
+  clear_error();
+  RopeAxesArgs a;
+  int rc = fill_rope_axes(a, B, S, Hq, Hk, D, positions, qw, kw, eps);
+  if (!rc) rc = put_rope_tensor("q_dout", q_dout, q_dout_strides, false, B, S, Hq, a.dys[0]);
+  if (!rc) rc = put_rope_tensor("k_dout", k_dout, k_dout_strides, false, B, S, Hk, a.dys[1]);
+  if (!rc) rc = put_rope_tensor("q", q, q_strides, false, B, S, Hq, a.xs[0]);
+  if (!rc) rc = put_rope_tensor("k", k, k_strides, false, B, S, Hk, a.xs[1]);
+  if (!rc) rc = put_rope_tensor("q_grad", q_grad, q_grad_strides, true, B, S, Hq, a.ys[0]);
+  if (!rc) rc = put_rope_tensor("k_grad", k_grad, k_grad_strides, true, B, S, Hk, a.ys[1]);
+  if (rc) return rc;
+  if (!qw_grad || !kw_grad) return fail(H3A_ERR_INVALID_ARG, "null weight gradient");
+  if ((reinterpret_cast<uintptr_t>(qw_grad) | reinterpret_cast<uintptr_t>(kw_grad)) & 3u)
+    return fail(H3A_ERR_ALIGNMENT, "weight gradients must be 4-byte aligned");
+  const size_t need = rope_axes_bwd_bytes(B, S);
+  if (!workspace || workspace_bytes < need)
+    return fail(H3A_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+  if (!aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  a.dy[0] = static_cast<const uint16_t *>(q_dout);
+  a.dy[1] = static_cast<const uint16_t *>(k_dout);
+  a.x[0] = static_cast<const uint16_t *>(q);
+  a.x[1] = static_cast<const uint16_t *>(k);
+  a.y[0] = static_cast<uint16_t *>(q_grad);
+  a.y[1] = static_cast<uint16_t *>(k_grad);
+  a.dw[0] = qw_grad;
+  a.dw[1] = kw_grad;
+  a.partial = static_cast<float *>(workspace);
+  return launch_rope_axes(a, true, as_stream(stream));
+}
+
+int h3a_layer_norm_fwd(const void *x, int64_t x_stride, const void *w, const void *b, void *y, int64_t y_stride,
+                       float *mean, float *rstd, int rows, int C, int dtype, int w_dtype, const int *bounds,
+                       int segments, int modulate, float eps, h3a_stream_t stream) {
+  clear_error();
+  int rc = check_norm(rows, C, dtype, w_dtype, bounds, segments);
+  if (rc) return rc;
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(H3A_ERR_INVALID_ARG, "eps must be finite and >= 0");
+  if (!mean != !rstd) return fail(H3A_ERR_INVALID_ARG, "mean and rstd come together");
+  NormArgs a = {};
+  bool vec = C % 8 == 0;
+  rc = norm_rows("x", x, x_stride, rows, C, dtype, false, &vec, &a.x_stride);
+  if (!rc) rc = norm_rows("y", y, y_stride, rows, C, dtype, true, &vec, &a.y_stride);
+  if (!rc) rc = norm_affine("w", w, w_dtype);
+  if (!rc) rc = norm_affine("b", b, w_dtype);
+  if (rc) return rc;
+  a.x = static_cast<const char *>(x);
+  a.y = static_cast<char *>(y);
+  a.w = w; a.b = b; a.w_dtype = w_dtype;
+  a.w_add = modulate ? 1.f : 0.f;
+  a.mean = mean; a.rstd = rstd;
+  a.C = C; a.eps = eps;
+  a.rows_per_wg = norm_rows_per_wg(rows, C, kNormFwdWgs);
+  return launch_layer_norm(a, bounds, segments, dtype, false, vec, as_stream(stream));
+}
+
+int h3a_layer_norm_bwd_workspace_size(const int *bounds, int segments, int C, size_t *bytes) {
+  clear_error();
+  if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
+  if (!bounds || segments <= 0) return fail(H3A_ERR_INVALID_ARG, "no segments");
+  const int rc = check_norm(bounds[segments], C, H3A_FP32, H3A_FP32, bounds, segments);
+  if (rc) return rc;
+  *bytes = norm_bwd_bytes(bounds, segments, C);
+  return H3A_OK;
+}
+
+int h3a_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *w,
+                       const float *mean, const float *rstd, void *dx, int64_t dx_stride, float *dw, float *db,
+                       int rows, int C, int dtype, int w_dtype, const int *bounds, int segments, int modulate,
+                       void *workspace, size_t workspace_bytes, h3a_stream_t stream) {
+  clear_error();
+  int rc = check_norm(rows, C, dtype, w_dtype, bounds, segments);
+  if (rc) return rc;
+  if (!dw != !db) return fail(H3A_ERR_INVALID_ARG, "dw and db come together");
+  NormArgs a = {};
+  bool vec = C % 8 == 0;
+  rc = norm_rows("dy", dy, dy_stride, rows, C, dtype, false, &vec, &a.dy_stride);
+  if (!rc) rc = norm_rows("x", x, x_stride, rows, C, dtype, false, &vec, &a.x_stride);
+  if (!rc) rc = norm_rows("dx", dx, dx_stride, rows, C, dtype, true, &vec, &a.y_stride);
+  if (!rc) rc = norm_affine("w", w, w_dtype);
+  if (rc) return rc;
+  if (rows > 0 && (!mean || !rstd)) return fail(H3A_ERR_INVALID_ARG, "null mean or rstd");
+  const size_t need = dw ? norm_bwd_bytes(bounds, segments, C) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(H3A_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+  if (need > 0 && !aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  a.dy = static_cast<const char *>(dy);
+  a.x = static_cast<const char *>(x);
+  a.y = static_cast<char *>(dx);
+  a.w = w; a.w_dtype = w_dtype;
+  a.w_add = modulate ? 1.f : 0.f;
+  a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+  a.dw = dw; a.db = db;
+  // Without rows no workgroup leaves a partial, and none is read; dw stands for "wanted".
+  a.partial = need > 0 ? static_cast<float *>(workspace) : dw;
+  a.C = C;
+  a.rows_per_wg = norm_rows_per_wg(rows, C, kNormBwdWgs);
+  return launch_layer_norm(a, bounds, segments, dtype, true, vec, as_stream(stream));
 }
 
 int h3a_kernel_attrs(int which, double out[6]) {

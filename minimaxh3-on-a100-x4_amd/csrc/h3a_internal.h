@@ -146,6 +146,52 @@ struct WindowArgs {
 int launch_window_fwd(WindowArgs a, hipStream_t s);
 int launch_window_bwd(WindowArgs a, hipStream_t s);
 
+// Kernel-side argument block of the layer norm kernels (h3a_norm.hip): up to
+// kNormSegments segments of rows per launch, whose workgroups are numbered on.
+constexpr int kNormSegments = 64;
+struct NormArgs {
+  const char *x, *dy;  // rows of C channels
+  char *y;             // forward: y; backward: dx
+  int64_t x_stride, dy_stride, y_stride;  // bytes from row to row
+  const void *w, *b;   // [segments, C], or null
+  int w_dtype;
+  float w_add;         // 1 for modulation, else 0
+  float *mean, *rstd;  // [rows]; forward: written unless null
+  float *partial;      // backward: [workgroups][2][C], or null
+  float *dw, *db;      // [segments, C]
+  int C, rows_per_wg, segments, seg0, wg0;
+  float eps;
+  int bounds[kNormSegments + 1], first_wg[kNormSegments + 1];
+};
+// Workgroups the rows are shared among: forward, and backward, where each leaves a
+// partial row of the weights' gradients.
+constexpr int kNormFwdWgs = 2048, kNormBwdWgs = 512;
+int norm_rows_per_wg(int64_t rows, int C, int wgs);
+int norm_wgs(const int *bounds, int segments, int rows_per_wg);
+int launch_layer_norm(NormArgs a, const int *bounds, int segments, int dtype, bool bwd, bool vec, hipStream_t s);
+
+// Argument block of the prologue from positions (h3a_prologue.hip).
+constexpr int kRopeAxes = 4;
+struct RopeAxesArgs {
+  const uint16_t *x[2];   // q, k [B,S,H,128]: strides {batch, seq, head}
+  const uint16_t *dy[2];  // backward: gradients of the outputs
+  uint16_t *y[2];         // forward: outputs; backward: gradients of x
+  int64_t xs[2][3], dys[2][3], ys[2][3];
+  const uint16_t *w[2];
+  int B, S, H[2];
+  const void *pos;  // [S, axes] or [B, S, axes], int32 or fp32
+  int pos_float, axes;
+  int64_t pos_b;    // elements from batch to batch (0: shared)
+  int rot;
+  float eps;
+  float *partial;   // backward: [workgroups][2][128]
+  float *dw[2];
+  double turns[64];   // revolutions per unit of position, pair by pair
+  uint8_t axis[64];
+};
+int rope_axes_bwd_wgs(int B, int S);
+int launch_rope_axes(const RopeAxesArgs &a, bool bwd, hipStream_t s);
+
 struct RopeArgs {
   uint16_t *q, *k;
   int64_t qsb, qss, qsh;

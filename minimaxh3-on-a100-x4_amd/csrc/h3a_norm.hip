@@ -1,0 +1,385 @@
+// Layer norm over rows of C channels, with a scale and shift per contiguous segment of
+// rows (the DiT's adaLN modulation of a packed sequence), forward and backward.
+//
+//   xhat = (x - mean) * rstd,  y = xhat * w + b,   w = weight, or 1 + weight (modulate)
+//   a = dy * w,  dx = rstd * (a - mean(a) - xhat * mean(a * xhat))
+//   dw = sum over the segment's rows of dy * xhat,  db = sum of dy
+//
+// Bound by HBM: every row is read once and written once.  A row is held in registers by
+// one wave (short rows) or one workgroup, 8 consecutive channels per thread and step;
+// a workgroup walks consecutive rows of one segment, so that the segment's weights, and
+// in the backward pass the sums of dw and db, stay in registers.  Those sums leave as
+// one fp32 partial row per workgroup and are added by a second kernel in a fixed order.
+// Statistics and sums are fp32; the variance is taken about the row's own mean.
+#include "h3a_device.h"
+#include "h3a_internal.h"
+
+namespace h3a {
+
+namespace {
+
+// 8 channels of a row, as they are in memory, and as floats.
+template <int DT>
+struct Row8 {
+  static constexpr int kBytes = DT == H3A_FP32 ? 4 : 2;
+  u32x4 v[DT == H3A_FP32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ float element(const char *p, int64_t i) {
+  if constexpr (DT == H3A_FP32) return reinterpret_cast<const float *>(p)[i];
+  else if constexpr (DT == H3A_FP16) return (float)reinterpret_cast<const _Float16 *>(p)[i];
+  else return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << 16);
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack(const Row8<DT> &r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == H3A_FP32) {
+      x[i] = __uint_as_float(r.v[0][i]);
+      x[i + 4] = __uint_as_float(r.v[1][i]);
+    } else if constexpr (DT == H3A_FP16) {
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+      const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)r.v[0][i]);
+      x[2 * i] = (float)h.x;
+      x[2 * i + 1] = (float)h.y;
+    } else {
+      x[2 * i] = bf16_lo(r.v[0][i]);
+      x[2 * i + 1] = bf16_hi(r.v[0][i]);
+    }
+  }
+}
+
+// Channels c .. c+7 of a row of C; those past the end are 0.  VEC: C is a multiple of 8
+// and rows are 16-byte aligned.
+template <int DT, bool VEC>
+__device__ __forceinline__ Row8<DT> load8(const char *row, int c, int C) {
+  Row8<DT> r;
+  if constexpr (VEC) {
+    constexpr int kVecs = sizeof(r.v) / sizeof(r.v[0]);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      r.v[i] = c < C ? *reinterpret_cast<const u32x4 *>(row + (int64_t)c * Row8<DT>::kBytes + 16 * i) : u32x4{0, 0, 0, 0};
+  } else if constexpr (DT == H3A_FP32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      r.v[i >> 2][i & 3] = c + i < C ? reinterpret_cast<const uint32_t *>(row)[c + i] : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t *p = reinterpret_cast<const uint16_t *>(row) + c + 2 * i;
+      const uint32_t lo = c + 2 * i < C ? p[0] : 0u, hi = c + 2 * i + 1 < C ? p[1] : 0u;
+      r.v[0][i] = lo | hi << 16;
+    }
+  }
+  return r;
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(char *row, int c, int C, const float (&x)[8]) {
+  Row8<DT> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == H3A_FP32) {
+      r.v[0][i] = __float_as_uint(x[i]);
+      r.v[1][i] = __float_as_uint(x[i + 4]);
+    } else if constexpr (DT == H3A_FP16) {
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+      r.v[0][i] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+    } else {
+      r.v[0][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    }
+  }
+  if constexpr (VEC) {
+    constexpr int kVecs = sizeof(r.v) / sizeof(r.v[0]);
+    if (c < C) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        *reinterpret_cast<u32x4 *>(row + (int64_t)c * Row8<DT>::kBytes + 16 * i) = r.v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (c + i >= C) break;
+      if constexpr (DT == H3A_FP32) reinterpret_cast<uint32_t *>(row)[c + i] = r.v[i >> 2][i & 3];
+      else reinterpret_cast<uint16_t *>(row)[c + i] = (uint16_t)(r.v[0][i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// A weight or bias row (bf16, fp16 or fp32, any alignment) as floats; it is read once
+// per workgroup and segment.
+__device__ __forceinline__ void load_affine(const void *p, int dt, int64_t row, int c, int C, float otherwise,
+                                            float add, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!p || c + i >= C) {
+      x[i] = otherwise;
+    } else {
+      const char *b = static_cast<const char *>(p);
+      const int64_t at = row * C + c + i;
+      x[i] = add + (dt == H3A_FP32 ? element<H3A_FP32>(b, at)
+                                   : dt == H3A_FP16 ? element<H3A_FP16>(b, at) : element<H3A_BF16>(b, at));
+    }
+  }
+}
+
+// Sums of two values over the TPR threads of a row, on all of them.  `slot` alternates
+// between rows, so that one barrier per row suffices.
+template <int TPR>
+__device__ __forceinline__ float2 row_sum(float2 v, float2 (*xch)[4], int slot) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    v.x += __shfl_xor(v.x, o);
+    v.y += __shfl_xor(v.y, o);
+  }
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) xch[slot][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = xch[slot][0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      v.x += xch[slot][w].x;
+      v.y += xch[slot][w].y;
+    }
+  }
+  return v;
+}
+
+// The workgroup's segment, and its rows [r0, r1) in it.
+struct Share {
+  int seg, r0, r1;
+};
+__device__ __forceinline__ Share share_of(const NormArgs &a) {
+  const int w = blockIdx.x;
+  int s = 0;
+  while (s + 1 < a.segments && w >= a.first_wg[s + 1]) ++s;
+  const int r0 = a.bounds[s] + (w - a.first_wg[s]) * a.rows_per_wg;
+  const int r1 = r0 + a.rows_per_wg;
+  return {s, r0, r1 < a.bounds[s + 1] ? r1 : a.bounds[s + 1]};
+}
+
+template <int DT, int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(256) layer_norm_fwd_kernel(NormArgs a) {
+  constexpr int kRowsAtOnce = 256 / TPR;
+  __shared__ float2 xch[4][4];
+  const int t = threadIdx.x % TPR;
+  const Share sh = share_of(a);
+  float w[NV][8], b[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (t + i * TPR);
+    load_affine(a.w, a.w_dtype, a.seg0 + sh.seg, c, a.C, 1.f, a.w_add, w[i]);
+    load_affine(a.b, a.w_dtype, a.seg0 + sh.seg, c, a.C, 0.f, 0.f, b[i]);
+  }
+  const float inv_c = 1.f / (float)a.C;
+  int slot = 0;
+  for (int r = sh.r0 + (int)threadIdx.x / TPR; r < sh.r1; r += kRowsAtOnce) {
+    const char *xr = a.x + (int64_t)r * a.x_stride;
+    float x[NV][8];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      unpack<DT>(load8<DT, VEC>(xr, 8 * (t + i * TPR), a.C), x[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += x[i][e];
+    }
+    const float mean = row_sum<TPR>(float2{sum, 0.f}, xch, slot).x * inv_c;
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[i][e] -= mean;
+        if (8 * (t + i * TPR) + e < a.C) sq = fmaf(x[i][e], x[i][e], sq);
+      }
+    const float rstd = rsqrtf(row_sum<TPR>(float2{sq, 0.f}, xch, slot + 1).x * inv_c + a.eps);
+    slot ^= 2;
+    if (t == 0 && a.mean) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+    char *yr = a.y + (int64_t)r * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = fmaf(x[i][e] * rstd, w[i][e], b[i][e]);
+      store8<DT, VEC>(yr, 8 * (t + i * TPR), a.C, y);
+    }
+  }
+}
+
+template <int DT, int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(256) layer_norm_bwd_kernel(NormArgs a) {
+  constexpr int kRowsAtOnce = 256 / TPR;
+  __shared__ float2 xch[2][4];
+  __shared__ float fold[TPR > 64 ? 1 : 3 * 64 * 8];
+  const int t = threadIdx.x % TPR;
+  const Share sh = share_of(a);
+  float w[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_affine(a.w, a.w_dtype, a.seg0 + sh.seg, 8 * (t + i * TPR), a.C, 1.f, a.w_add, w[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
+  }
+  const float inv_c = 1.f / (float)a.C;
+  int slot = 0;
+  for (int r = sh.r0 + (int)threadIdx.x / TPR; r < sh.r1; r += kRowsAtOnce) {
+    const char *xr = a.x + (int64_t)r * a.x_stride, *gr = a.dy + (int64_t)r * a.dy_stride;
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    float xh[NV][8], g[NV][8];
+    float2 s = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (t + i * TPR);
+      unpack<DT>(load8<DT, VEC>(xr, c, a.C), xh[i]);
+      unpack<DT>(load8<DT, VEC>(gr, c, a.C), g[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xh[i][e] = (xh[i][e] - mean) * rstd;
+        dw[i][e] = fmaf(g[i][e], xh[i][e], dw[i][e]);
+        db[i][e] += g[i][e];
+        g[i][e] *= w[i][e];
+        s.x += g[i][e];
+        s.y = fmaf(g[i][e], xh[i][e], s.y);
+      }
+    }
+    s = row_sum<TPR>(s, xch, slot);
+    slot ^= 1;
+    const float m1 = s.x * inv_c, m2 = s.y * inv_c;
+    char *dr = a.y + (int64_t)r * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float d[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = rstd * (g[i][e] - m1 - xh[i][e] * m2);
+      store8<DT, VEC>(dr, 8 * (t + i * TPR), a.C, d);
+    }
+  }
+  if (!a.partial) return;
+  float *out = a.partial + (int64_t)(a.wg0 + blockIdx.x) * 2 * a.C;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float(&v)[8] = which ? db[i] : dw[i];
+      if constexpr (TPR == 64) {  // the other waves' rows
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();
+        if (wave > 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) fold[((wave - 1) * 8 + e) * 64 + t] = v[e];
+        }
+        __syncthreads();
+        if (wave > 0) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (v[e] + fold[e * 64 + t]) + (fold[(8 + e) * 64 + t] + fold[(16 + e) * 64 + t]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = 8 * (t + i * TPR) + e;
+        if (c < a.C) out[which * a.C + c] = v[e];
+      }
+    }
+  }
+}
+
+// Sums of the partial rows of each segment's workgroups: 64 channels of dw or db per
+// workgroup, its four waves taking every fourth row.
+__global__ void __launch_bounds__(256) layer_norm_param_grad_kernel(NormArgs a) {
+  __shared__ float fold[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane, seg = blockIdx.y, which = blockIdx.z;
+  const int w0 = a.wg0 + a.first_wg[seg], w1 = a.wg0 + a.first_wg[seg + 1];
+  float sum = 0.f;
+  if (c < a.C)
+    for (int w = w0 + wave; w < w1; w += 4) sum += a.partial[((int64_t)w * 2 + which) * a.C + c];
+  fold[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && c < a.C)
+    (which ? a.db : a.dw)[(int64_t)(a.seg0 + seg) * a.C + c] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
+}
+
+typedef void (*NormKernel)(NormArgs);
+
+// Rows up to 1024 channels take one wave, longer ones a workgroup.
+template <int DT, bool VEC>
+NormKernel pick_fwd(int C, int *rows_at_once) {
+  *rows_at_once = C <= 1024 ? 4 : 1;
+  if (C <= 512) return layer_norm_fwd_kernel<DT, 64, 1, VEC>;
+  if (C <= 1024) return layer_norm_fwd_kernel<DT, 64, 2, VEC>;
+  if (C <= 2048) return layer_norm_fwd_kernel<DT, 256, 1, VEC>;
+  if (C <= 4096) return layer_norm_fwd_kernel<DT, 256, 2, VEC>;
+  if (C <= 6144) return layer_norm_fwd_kernel<DT, 256, 3, VEC>;
+  if (C <= 8192) return layer_norm_fwd_kernel<DT, 256, 4, VEC>;
+  return layer_norm_fwd_kernel<DT, 256, 8, VEC>;
+}
+template <int DT, bool VEC>
+NormKernel pick_bwd(int C, int *rows_at_once) {
+  *rows_at_once = C <= 1024 ? 4 : 1;
+  if (C <= 512) return layer_norm_bwd_kernel<DT, 64, 1, VEC>;
+  if (C <= 1024) return layer_norm_bwd_kernel<DT, 64, 2, VEC>;
+  if (C <= 2048) return layer_norm_bwd_kernel<DT, 256, 1, VEC>;
+  if (C <= 4096) return layer_norm_bwd_kernel<DT, 256, 2, VEC>;
+  if (C <= 6144) return layer_norm_bwd_kernel<DT, 256, 3, VEC>;
+  if (C <= 8192) return layer_norm_bwd_kernel<DT, 256, 4, VEC>;
+  return layer_norm_bwd_kernel<DT, 256, 8, VEC>;
+}
+template <bool BWD, bool VEC>
+NormKernel pick(int dtype, int C, int *rows_at_once) {
+  switch (dtype) {
+    case H3A_FP32: return BWD ? pick_bwd<H3A_FP32, VEC>(C, rows_at_once) : pick_fwd<H3A_FP32, VEC>(C, rows_at_once);
+    case H3A_FP16: return BWD ? pick_bwd<H3A_FP16, VEC>(C, rows_at_once) : pick_fwd<H3A_FP16, VEC>(C, rows_at_once);
+    default: return BWD ? pick_bwd<H3A_BF16, VEC>(C, rows_at_once) : pick_fwd<H3A_BF16, VEC>(C, rows_at_once);
+  }
+}
+
+}  // namespace
+
+// Rows per workgroup: so many that `wgs` workgroups share all the rows (each segment
+// adds at most one more), in whole steps of the rows it takes at once.
+int norm_rows_per_wg(int64_t rows, int C, int wgs) {
+  const int step = C <= 1024 ? 4 : 1;
+  const int64_t n = (rows + wgs - 1) / wgs;
+  return (int)((n < 1 ? 1 : n) + step - 1) / step * step;
+}
+
+int norm_wgs(const int *bounds, int segments, int rows_per_wg) {
+  int64_t n = 0;
+  for (int s = 0; s < segments; ++s) n += (bounds[s + 1] - bounds[s] + rows_per_wg - 1) / rows_per_wg;
+  return (int)n;
+}
+
+int launch_layer_norm(NormArgs a, const int *bounds, int segments, int dtype, bool bwd, bool vec, hipStream_t s) {
+  int at_once = 1;
+  const NormKernel kernel = bwd ? (vec ? pick<true, true>(dtype, a.C, &at_once) : pick<true, false>(dtype, a.C, &at_once))
+                                : (vec ? pick<false, true>(dtype, a.C, &at_once) : pick<false, false>(dtype, a.C, &at_once));
+  a.wg0 = 0;
+  for (a.seg0 = 0; a.seg0 < segments; a.seg0 += kNormSegments) {
+    a.segments = segments - a.seg0 < kNormSegments ? segments - a.seg0 : kNormSegments;
+    int wgs = 0;
+    for (int i = 0; i <= a.segments; ++i) {
+      a.bounds[i] = bounds[a.seg0 + i];
+      a.first_wg[i] = wgs;
+      if (i < a.segments) wgs += (bounds[a.seg0 + i + 1] - a.bounds[i] + a.rows_per_wg - 1) / a.rows_per_wg;
+    }
+    if (wgs > 0) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(256), 0, s, a);
+      const int rc = check_launch(bwd ? "layer_norm_bwd_kernel" : "layer_norm_fwd_kernel");
+      if (rc) return rc;
+    }
+    if (bwd && a.partial) {
+      hipLaunchKernelGGL(layer_norm_param_grad_kernel, dim3((unsigned)((a.C + 63) / 64), (unsigned)a.segments, 2),
+                         dim3(256), 0, s, a);
+      const int rc = check_launch("layer_norm_param_grad_kernel");
+      if (rc) return rc;
+    }
+    a.wg0 += wgs;
+  }
+  return H3A_OK;
+}
+
+}  // namespace h3a

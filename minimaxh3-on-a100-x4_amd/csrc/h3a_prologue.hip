@@ -342,6 +342,196 @@ int launch_qk_rmsnorm_rope(const RopeArgs &a, hipStream_t s) {
   return check_launch("qk_rmsnorm_rope_kernel");
 }
 
+// ---------------------------------------------------------------------------
+// The prologue from positions on several axes (time, height, width), out of place or in
+// place, and its backward pass.  Pair i of a token turns by pos[axis(i)] * turns[i]
+// revolutions; with y' = R(angle) (x * r * w), r = rsqrt(mean(x^2) + eps):
+//   g = R(angle)^T dy',  dw = sum over rows of g * x * r,
+//   dx = r * (g * w - x * r^2 * mean(x * g * w))
+// HBM-bound as the kernel above, and laid out like it: 16 lanes per head row, 8 dims per
+// lane.  The angles of four tokens are taken once per workgroup, one pair per lane, and
+// shared through LDS: the product with the position in fp64 (exact to 2^-53 of the
+// angle: far positions lose nothing), its fraction of a revolution in fp32.
+__device__ __forceinline__ void token_angles(const RopeAxesArgs &a, int64_t bs, int lane, float (*cs)[64]) {
+  if (2 * lane < a.rot) {
+    const int64_t at = bs / a.S * a.pos_b + bs % a.S * a.axes + a.axis[lane];
+    const double pos = a.pos_float ? (double)static_cast<const float *>(a.pos)[at]
+                                   : (double)static_cast<const int32_t *>(a.pos)[at];
+    double t = pos * a.turns[lane];
+    t -= __builtin_rint(t);
+    float s, c;
+    sincospif((float)(2.0 * t), &s, &c);
+    cs[0][lane] = c;
+    cs[1][lane] = s;
+  }
+}
+
+// The lane's 8 cosines and sines; its dims are 8c .. 8c+7, nh lanes hold a half.  The
+// second half's sine is the first's negated: y'_c = cos y_c - sgn sin y_partner.
+__device__ __forceinline__ void lane_angles(const float (*cs)[64], int c, int nh, float (&co)[8], float (&si)[8]) {
+  const int f = c < nh ? c : c - nh;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    co[e] = c < 2 * nh ? cs[0][8 * f + e] : 1.f;
+    si[e] = c < 2 * nh ? (c < nh ? -cs[1][8 * f + e] : cs[1][8 * f + e]) : 0.f;
+  }
+}
+
+// x[e] of the lane that holds the other dim of each pair.
+template <bool kRot128>
+__device__ __forceinline__ void partner8(const float (&x)[8], float (&xp)[8], int c, int nh) {
+  if (kRot128) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) xp[e] = dpp_row<kDppRor8>(x[e]);
+  } else {
+    const int partner = c < nh ? c + nh : (c < 2 * nh ? c - nh : c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) xp[e] = __shfl(x[e], partner, 16);
+  }
+}
+
+constexpr int kAxesTokens = 4;  // tokens per workgroup and step
+
+// kSteps: head rows per lane group in flight, so kSteps * 4 heads per item; items of a
+// step are (token, tensor, chunk of heads), dealt to the workgroup's four waves.
+template <int kSteps, bool kRot128, bool kBwd>
+__global__ void __launch_bounds__(256) rope_axes_kernel(RopeAxesArgs a) {
+  __shared__ float angles[2][kAxesTokens][2][64];
+  __shared__ float fold[kBwd ? 4 : 1][2][128];
+  const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nh = a.rot >> 4;
+  const int64_t tokens = (int64_t)a.B * a.S;
+  const int chunks[2] = {(a.H[0] + 4 * kSteps - 1) / (4 * kSteps), (a.H[1] + 4 * kSteps - 1) / (4 * kSteps)};
+  const int per_token = chunks[0] + chunks[1];
+  float dw[2][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = 0.f;
+  int slot = 0;
+  for (int64_t t0 = (int64_t)blockIdx.x * kAxesTokens; t0 < tokens; t0 += (int64_t)gridDim.x * kAxesTokens) {
+    if (t0 + wave < tokens) token_angles(a, t0 + wave, lane, angles[slot][wave]);
+    __syncthreads();
+    for (int item = wave; item < kAxesTokens * per_token; item += 4) {
+      const int64_t bs = t0 + item / per_token;
+      if (bs >= tokens) break;
+      int chunk = item % per_token;
+      const int which = chunk < chunks[0] ? 0 : 1;
+      chunk -= which ? chunks[0] : 0;
+      const int H = which ? a.H[1] : a.H[0], h0 = chunk * 4 * kSteps;
+      const int64_t b = bs / a.S, s = bs % a.S;
+      const int64_t *xs = which ? a.xs[1] : a.xs[0], *ys = which ? a.ys[1] : a.ys[0];
+      const uint16_t *xrow = (which ? a.x[1] : a.x[0]) + b * xs[0] + s * xs[1] + 8 * c;
+      uint16_t *yrow = (which ? a.y[1] : a.y[0]) + b * ys[0] + s * ys[1] + 8 * c;
+      u32x4 xv[kSteps], gv[kBwd ? kSteps : 1];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int h = h0 + 4 * i + grp < H ? h0 + 4 * i + grp : H - 1;
+        xv[i] = *(const u32x4 *)(xrow + h * xs[2]);
+        if constexpr (kBwd) {
+          const int64_t *gs = which ? a.dys[1] : a.dys[0];
+          gv[i] = *(const u32x4 *)((which ? a.dy[1] : a.dy[0]) + b * gs[0] + s * gs[1] + 8 * c + h * gs[2]);
+        }
+      }
+      float w[8], co[8], si[8];
+      unpack8(*(const u32x4 *)((which ? a.w[1] : a.w[0]) + 8 * c), w);
+      lane_angles(angles[slot][item / per_token], c, nh, co, si);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (h0 + 4 * i >= H) break;
+        const int h = h0 + 4 * i + grp;
+        float x[8], p[8], y[8];
+        unpack8(xv[i], x);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        const float r = rsqrtf(group16_sum(ss) * (1.0f / kRopeD) + a.eps);
+        if constexpr (!kBwd) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+          partner8<kRot128>(x, p, c, nh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fmaf(co[e], x[e], si[e] * p[e]);
+        } else {
+          float g[8], m = 0.f;
+          unpack8(gv[i], g);
+          partner8<kRot128>(g, p, c, nh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            g[e] = fmaf(co[e], g[e], -si[e] * p[e]);
+            const float gx = g[e] * x[e];
+            if (h < H) {
+              if (which) dw[1][e] = fmaf(gx, r, dw[1][e]);
+              else dw[0][e] = fmaf(gx, r, dw[0][e]);
+            }
+            m = fmaf(gx, w[e], m);
+          }
+          m = group16_sum(m) * (1.0f / kRopeD) * r * r;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = r * fmaf(-x[e], m, g[e] * w[e]);
+        }
+        if (h < H) *(u32x4 *)(yrow + h * ys[2]) = pack8(y);
+      }
+    }
+    slot ^= 1;
+  }
+  if constexpr (kBwd) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = dw[which][e];
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        if (grp == 0) fold[wave][which][8 * c + e] = v;
+      }
+    __syncthreads();
+    const int which = tid >> 7, d = tid & 127;
+    a.partial[(int64_t)blockIdx.x * 256 + tid] =
+        (fold[0][which][d] + fold[1][which][d]) + (fold[2][which][d] + fold[3][which][d]);
+  }
+}
+
+// Sums of the workgroups' partial rows in a fixed order: 16 columns per workgroup, 16
+// lanes to a column, each taking every sixteenth row.
+__global__ void __launch_bounds__(256) rope_axes_param_grad_kernel(RopeAxesArgs a, int wgs) {
+  __shared__ float fold[16][17];
+  const int col = threadIdx.x & 15, part = threadIdx.x >> 4, at = blockIdx.x * 16 + col;
+  float sum = 0.f;
+  for (int i = part; i < wgs; i += 16) sum += a.partial[(int64_t)i * 256 + at];
+  fold[part][col] = sum;
+  __syncthreads();
+  if (part == 0) {
+    sum = 0.f;
+    for (int i = 0; i < 16; ++i) sum += fold[i][col];
+    a.dw[at >> 7][at & 127] = sum;
+  }
+}
+
+// Backward: workgroups that each leave a partial row of the weights' gradients.
+int rope_axes_bwd_wgs(int B, int S) {
+  const int64_t n = ((int64_t)B * S + kAxesTokens - 1) / kAxesTokens;
+  return (int)(n < 1024 ? n : 1024);
+}
+
+template <bool kBwd>
+static int launch_rope_axes_as(const RopeAxesArgs &a, hipStream_t s) {
+  const int64_t groups = ((int64_t)a.B * a.S + kAxesTokens - 1) / kAxesTokens;
+  const int64_t wgs = kBwd ? rope_axes_bwd_wgs(a.B, a.S) : groups;
+  const bool full = a.rot == kRopeD;
+  const int h = a.H[0] > a.H[1] ? a.H[0] : a.H[1];
+  void (*kernel)(RopeAxesArgs) =
+      h > 16 ? (full ? rope_axes_kernel<7, true, kBwd> : rope_axes_kernel<7, false, kBwd>)
+             : (full ? rope_axes_kernel<2, true, kBwd> : rope_axes_kernel<2, false, kBwd>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(256), 0, s, a);
+  int rc = check_launch("rope_axes_kernel");
+  if (rc || !kBwd) return rc;
+  hipLaunchKernelGGL(rope_axes_param_grad_kernel, dim3(16), dim3(256), 0, s, a, (int)wgs);
+  return check_launch("rope_axes_param_grad_kernel");
+}
+int launch_rope_axes(const RopeAxesArgs &a, bool bwd, hipStream_t s) {
+  return bwd ? launch_rope_axes_as<true>(a, s) : launch_rope_axes_as<false>(a, s);
+}
+
 int rope_kernel_attrs(double out[6]) {
   hipFuncAttributes fa;
   const void *fn = reinterpret_cast<const void *>(&qk_rmsnorm_rope_kernel<28, true>);  // the H=56 width

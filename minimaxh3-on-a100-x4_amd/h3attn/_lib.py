@@ -25,6 +25,8 @@ H3A_ERR_UNSUPPORTED = 2
 H3A_ERR_ALIGNMENT = 3
 H3A_ERR_HIP = 4
 
+BF16, FP16, FP32 = 0, 1, 2
+
 KERNEL_ATTN_DENSE = 0
 KERNEL_ATTN_SPARSE_128 = 1
 KERNEL_ATTN_SPARSE_64 = 2
@@ -42,6 +44,15 @@ class Window(ctypes.Structure):
     """h3a_window."""
     _fields_ = [("left", _i), ("right", _i), ("sinks", _i), ("causal", _i), ("q_start", _i), ("q_starts", _vp),
                 ("kv_lens", _vp)]
+
+
+MAX_AXES = 4
+
+
+class Positions(ctypes.Structure):
+    """h3a_positions."""
+    _fields_ = [("pos", _vp), ("batch_stride", _i64), ("pos_float", _i), ("axes", _i), ("dims", _i * MAX_AXES),
+                ("theta", ctypes.c_double)]
 
 
 # Every symbol of include/h3attn.h with its (restype, argtypes).
@@ -82,6 +93,16 @@ SIGNATURES = {
                                  _vp, _i64, _i64, _i, _vp, _vp, _f, _vp]),
     "h3a_qk_rmsnorm_rope_pool": (_i, [_vp, _vp, _i, _i, _i, _i, _c_i64_3, _c_i64_3,
                                       _vp, _i64, _i64, _i, _vp, _vp, _f, _i, _vp, _vp, _vp]),
+    "h3a_qk_rmsnorm_rope_axes": (_i, [_vp] * 4 + [_i] * 5 + [_c_i64_3] * 4 + [ctypes.POINTER(Positions), _vp, _vp,
+                                                                              _f, _vp]),
+    "h3a_qk_rmsnorm_rope_axes_bwd_workspace_size": (_i, [_i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "h3a_qk_rmsnorm_rope_axes_bwd": (_i, [_vp] * 8 + [_i] * 5 + [_c_i64_3] * 6 + [ctypes.POINTER(Positions), _vp,
+                                                                                  _vp, _f, _vp, ctypes.c_size_t, _vp]),
+    "h3a_layer_norm_fwd": (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(_i), _i, _i,
+                                _f, _vp]),
+    "h3a_layer_norm_bwd_workspace_size": (_i, [ctypes.POINTER(_i), _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "h3a_layer_norm_bwd": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i,
+                                ctypes.POINTER(_i), _i, _i, _vp, ctypes.c_size_t, _vp]),
     "h3a_block_pool": (_i, [_vp, _i, _i, _i, _i, _c_i64_3, _i, _vp, _vp]),
     "h3a_block_select": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "h3a_kernel_attrs": (_i, [_i, ctypes.POINTER(ctypes.c_double)]),
