@@ -263,7 +263,8 @@ int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, fl
  * bits.  workspace: h3a_attn_bwd_window_workspace_size bytes, untouched until the
  * call's work has completed.
  */
-int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, size_t *bytes);
+int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D,
+                                       const h3a_window *window, size_t *bytes);
 int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const void *v, const void *o,
                         const float *lse, void *dq, void *dk, void *dv,
                         int B, int H, int Hkv, int Sq, int Skv, int D,

@@ -292,8 +292,6 @@ size_t norm_bwd_bytes(const int *bounds, int segments, int C) {
   return (size_t)wgs * 2 * C * sizeof(float);
 }
 
-size_t window_bwd_bytes(int B, int H, int Sq) { return (size_t)B * H * Sq * sizeof(float); }
-
 }  // namespace
 }  // namespace h3a
 
@@ -589,12 +587,16 @@ int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, fl
   return launch_window_fwd(a, as_stream(stream));
 }
 
-int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, size_t *bytes) {
+int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, const h3a_window *window,
+                                       size_t *bytes) {
   clear_error();
   if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
-  const int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
+  int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
+  if (!rc) rc = check_window(window, Sq, Skv, 1.f);
   if (rc) return rc;
-  *bytes = window_bwd_bytes(B, H, Sq);
+  WindowArgs a;
+  fill_window_args(a, B, H, Hkv, Sq, Skv, *window, 1.f);
+  *bytes = window_bwd_bytes(a);
   return H3A_OK;
 }
 
@@ -619,12 +621,12 @@ int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const vo
   if (rc) return rc;
   if (!lse) return fail(H3A_ERR_INVALID_ARG, "null lse");
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(H3A_ERR_ALIGNMENT, "lse must be 4-byte aligned");
-  const size_t need = window_bwd_bytes(B, H, Sq);
+  WindowArgs a;
+  fill_window_args(a, B, H, Hkv, Sq, Skv, *window, scale);
+  const size_t need = window_bwd_bytes(a);
   if (!workspace || workspace_bytes < need)
     return fail(H3A_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
   if (!aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  WindowArgs a;
-  fill_window_args(a, B, H, Hkv, Sq, Skv, *window, scale);
   a.q = static_cast<const uint16_t *>(q);
   a.k = static_cast<const uint16_t *>(k);
   a.v = static_cast<const uint16_t *>(v);
@@ -634,7 +636,6 @@ int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const vo
   a.dq = static_cast<uint16_t *>(dq);
   a.dk = static_cast<uint16_t *>(dk);
   a.dv = static_cast<uint16_t *>(dv);
-  a.delta = static_cast<float *>(workspace);
   put_strides(a.gsb, a.gsh, a.gss, dout_strides, Sq);
   put_strides(a.qsb, a.qsh, a.qss, q_strides, Sq);
   put_strides(a.ksb, a.ksh, a.kss, k_strides, Skv);
@@ -643,7 +644,7 @@ int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const vo
   put_strides(a.dqsb, a.dqsh, a.dqss, dq_strides, Sq);
   put_strides(a.dksb, a.dksh, a.dkss, dk_strides, Skv);
   put_strides(a.dvsb, a.dvsh, a.dvss, dv_strides, Skv);
-  return launch_window_bwd(a, as_stream(stream));
+  return launch_window_bwd(a, workspace, as_stream(stream));
 }
 
 int h3a_block_map_to_tile_lut(const uint8_t *block_map, int B, int H, int Sq, int Skv, int blk_q, int blk_k,

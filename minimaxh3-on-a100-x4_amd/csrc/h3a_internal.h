@@ -142,9 +142,12 @@ struct WindowArgs {
   int64_t dksb, dksh, dkss;
   int64_t dvsb, dvsh, dvss;
   float *delta;  // [B,H,Sq] dO.O
+  int first_tiles, pieces;  // key tiles cut into runs of queries, and the runs of each
+  float *part;              // their partial sums: [B,Hkv,first_tiles,pieces][dK, dV][128][128]
 };
 int launch_window_fwd(WindowArgs a, hipStream_t s);
-int launch_window_bwd(WindowArgs a, hipStream_t s);
+int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s);
+size_t window_bwd_bytes(WindowArgs a);  // workspace, from the sizes and the window
 
 // Kernel-side argument block of the layer norm kernels (h3a_norm.hip): up to
 // kNormSegments segments of rows per launch, whose workgroups are numbered on.

@@ -337,16 +337,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 // Backward, dK and dV: a workgroup takes 128 keys of one key head, a wave 32 of them as
 // columns, and streams the queries that see them, of every head that shares the keys,
-// in 32-row stages of Q and dO.  A key's queries are one interval of positions, so the
+// in 64-row stages of Q and dO.  A key's queries are one interval of positions, so the
 // sums run in a fixed order with no atomics.
+//
+// The first keys are seen by every query, the others by a window's: tiles that hold
+// first keys are cut into a.pieces equal runs of stages, which leave fp32 partial sums
+// in a.part for window_dkdv_sum_kernel.
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dkdv_kernel(WindowArgs a) {
   using L = DualLayout;
-  constexpr int kQ = 32;  // queries per stage
+  constexpr int kQ = 64;  // queries per stage
   __shared__ __attribute__((aligned(16))) uint16_t qbuf[2][kQ * 128], dbuf[2][kQ * 128];
   __shared__ __attribute__((aligned(16))) float stats[2][2][kQ];  // lse (log2 units), delta
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Item it = item_of(a.total, a.nkt, a.Hkv);
+  const int first_items = a.first_tiles * a.pieces, per_bh = a.nkt - a.first_tiles + first_items;
+  Item it = item_of(a.total, per_bh, a.Hkv);
+  int piece = -1;  // of tile it.tile
+  if (it.tile < first_items) {
+    piece = it.tile % a.pieces;
+    it.tile /= a.pieces;
+  } else {
+    it.tile -= first_items - a.first_tiles;
+  }
   const Span sp = span_of(a, it.b);
   const int j0 = it.tile * kRows, wj0 = j0 + 32 * wave, key = wj0 + l32;
   const int j1 = (j0 + kRows < sp.len ? j0 + kRows : sp.len) - 1;
@@ -362,7 +374,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   } else if (a.causal) {
     i_a = j0 - sp.qs > i_a ? j0 - sp.qs : i_a;
   }
-  if (j1 >= j0 && i_b > i_a) {
+  // Stage t: rows i0 .. of head h; stages t_a .. t_b - 1 are this piece's.
+  const int per_head = j1 >= j0 && i_b > i_a ? (i_b - i_a + kQ - 1) / kQ : 0;
+  const int64_t stages = (int64_t)per_head * a.rep;
+  const int64_t t_a = piece < 0 ? 0 : stages * piece / a.pieces;
+  const int64_t t_b = piece < 0 ? stages : stages * (piece + 1) / a.pieces;
+  if (t_b > t_a) {
     // Positions that see the lane's key.
     int plo = key - a.right, phi = key + a.left;
     if (key < a.sinks) {
@@ -377,53 +394,56 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     TileDma<4, L, false, kQ> qdma, ddma;
     qdma.init(a.qss, wave, lane);
     ddma.init(a.gss, wave, lane);
-    const int per_head = (i_b - i_a + kQ - 1) / kQ, total = per_head * a.rep;
-    // Stage t: rows i0 .. of head h; the next one is fetched while it runs.
-    int h = it.h * a.rep, i0 = i_a;
+    int h = it.h * a.rep + (int)(t_a / per_head), i0 = i_a + (int)(t_a % per_head) * kQ;
     float st_next = 0.f;
     auto fetch = [&](int buf) __attribute__((always_inline)) {
       qdma.issue(a.q + it.b * a.qsb + h * a.qsh, a.qss, i0, i_b, qbuf[buf]);
       ddma.issue(a.dout + it.b * a.gsb + h * a.gsh, a.gss, i0, i_b, dbuf[buf]);
-      // Threads 0-31 take the rows' lse, 32-63 their delta; rows past the end get p = 0.
-      if (tid < 2 * kQ) {
-        const int i = i0 + (tid & 31);
+      // Waves 0 and 1 take the rows' lse and delta; rows past the end get p = 0.
+      if (wave < 2) {
+        const int i = i0 + lane;
         const int64_t at = ((int64_t)it.b * a.H + h) * a.Sq + (i < i_b ? i : i_b - 1);
-        const float x = tid < kQ ? a.lse[at] : a.delta[at];
-        if (tid < kQ) st_next = i < i_b && x != kNegInf ? x * kLog2e : -kNegInf;
+        const float x = wave == 0 ? a.lse[at] : a.delta[at];
+        if (wave == 0) st_next = i < i_b && x != kNegInf ? x * kLog2e : -kNegInf;
         else st_next = i < i_b ? x : 0.f;
       }
     };
     fetch(0);
-    if (tid < 2 * kQ) stats[0][tid >> 5][tid & 31] = st_next;
+    if (wave < 2) stats[0][wave][lane] = st_next;
     const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
     wait_vmem_all();
     __syncthreads();
+    const int total = (int)(t_b - t_a);
     for (int t = 0; t < total; ++t) {
-      const int buf = t & 1, p0 = sp.qs + i0, p1 = p0 + kQ - 1, rows = i_b - i0;
+      const int buf = t & 1, p_stage = sp.qs + i0, rows = i_b - i0;
       i0 += kQ;
       if (i0 >= i_b) {
         i0 = i_a;
         ++h;
       }
       if (t + 1 < total) fetch(buf ^ 1);
-      bool none, all = keys_whole && rows >= kQ;
-      if (wj0 < a.sinks) {
-        none = a.causal && p1 < wj0;
-        if (wj0 + 31 >= a.sinks) all = all && p0 >= wj0 + 31 - a.right && p1 <= a.sinks + a.left;
-        else all = all && (!a.causal || p0 >= wj0 + 31);
-      } else {
-        none = p1 < wj0 - a.right || p0 > wj0 + 31 + a.left;
-        all = all && p0 >= wj0 + 31 - a.right && p1 <= wj0 + a.left;
-      }
-      if (!none) {
+#pragma unroll 1  // one 32-row half's registers at a time
+      for (int u = 0; u < kQ / 32; ++u) {
+        const int p0 = p_stage + 32 * u, p1 = p0 + 31;
+        bool none = rows <= 32 * u, all = keys_whole && rows >= 32 * u + 32;
+        if (wj0 < a.sinks) {
+          none = none || (a.causal && p1 < wj0);
+          if (wj0 + 31 >= a.sinks) all = all && p0 >= wj0 + 31 - a.right && p1 <= a.sinks + a.left;
+          else all = all && (!a.causal || p0 >= wj0 + 31);
+        } else {
+          none = none || p1 < wj0 - a.right || p0 > wj0 + 31 + a.left;
+          all = all && p0 >= wj0 + 31 - a.right && p1 <= wj0 + a.left;
+        }
+        if (none) continue;
+        const uint16_t *qt = qbuf[buf] + u * 32 * 128, *dt = dbuf[buf] + u * 32 * 128;
         f32x16 s[1], dp[1];
         u32x4 pf[2], dsf[2];
-        score_tile<L, 1>(qbuf[buf], kf, k_rd, s);
-        score_tile<L, 1>(dbuf[buf], vf, k_rd, dp);
+        score_tile<L, 1>(qt, kf, k_rd, s);
+        score_tile<L, 1>(dt, vf, k_rd, dp);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const float4 l2 = *(const float4 *)&stats[buf][0][8 * r4 + 4 * g];
-          const float4 de = *(const float4 *)&stats[buf][1][8 * r4 + 4 * g];
+          const float4 l2 = *(const float4 *)&stats[buf][0][32 * u + 8 * r4 + 4 * g];
+          const float4 de = *(const float4 *)&stats[buf][1][32 * u + 8 * r4 + 4 * g];
           const float lv[4] = {l2.x, l2.y, l2.z, l2.w}, dl[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -437,22 +457,76 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
         pack_p<1>(s, pf);
         pack_p<1>(dp, dsf);
-        transposed_product<2>(dbuf[buf], pf, t_rd, dv);
-        transposed_product<2>(qbuf[buf], dsf, t_rd, dk);
+        transposed_product<2>(dt, pf, t_rd, dv);
+        transposed_product<2>(qt, dsf, t_rd, dk);
       }
-      if (t + 1 < total && tid < 2 * kQ) stats[buf ^ 1][tid >> 5][tid & 31] = st_next;
+      if (t + 1 < total && wave < 2) stats[buf ^ 1][wave][lane] = st_next;
       wait_vmem_all();
       __syncthreads();
     }
   }
-  if (wj0 < a.Skv) {
+  if (piece >= 0) {
+    const int64_t bh = (int64_t)it.b * a.Hkv + it.h;
+    float *part = a.part + ((bh * a.first_tiles + it.tile) * a.pieces + piece) * (2 * kRows * 128) +
+                  (32 * wave + l32) * 128 + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) {
+        *(float4 *)(part + dt * 32 + 8 * rr) =
+            float4{dk[dt][4 * rr], dk[dt][4 * rr + 1], dk[dt][4 * rr + 2], dk[dt][4 * rr + 3]};
+        *(float4 *)(part + kRows * 128 + dt * 32 + 8 * rr) =
+            float4{dv[dt][4 * rr], dv[dt][4 * rr + 1], dv[dt][4 * rr + 2], dv[dt][4 * rr + 3]};
+      }
+  } else if (wj0 < a.Skv) {
     const bool live = key < sp.len;
-    uint8_t *tile = reinterpret_cast<uint8_t *>(wave < 2 ? &qbuf[0][0] : &dbuf[0][0]) + (wave & 1) * 8192;
+    uint8_t *tile = reinterpret_cast<uint8_t *>(&qbuf[0][0]) + wave * 8192;
     store_columns(dk, a.scale, live, tile, a.dk + it.b * a.dksb + it.h * a.dksh + (int64_t)wj0 * a.dkss, a.dkss,
                   a.Skv - wj0, lane);
     store_columns(dv, 1.f, live, tile, a.dv + it.b * a.dvsb + it.h * a.dvsh + (int64_t)wj0 * a.dvss, a.dvss,
                   a.Skv - wj0, lane);
   }
+}
+
+// dK and dV of the tiles that were cut: the pieces' partial sums in order.  A thread
+// takes 4 dims of a key.
+__global__ void __launch_bounds__(256) window_dkdv_sum_kernel(WindowArgs a) {
+  const int rows = a.first_tiles * kRows, d = 4 * (threadIdx.x & 31);
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // ((b, h), dk or dv, key)
+  const int key = (int)(item % rows), which = (int)(item / rows & 1);
+  const int64_t bh = item / rows / 2;
+  if (key >= a.Skv || bh >= (int64_t)a.B * a.Hkv) return;
+  const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
+  const float *p = a.part + ((bh * a.first_tiles + key / kRows) * a.pieces * 2 + which) * (kRows * 128) +
+                   (key % kRows) * 128 + d;
+  float4 sum = *(const float4 *)p;
+  for (int i = 1; i < a.pieces; ++i) {
+    const float4 x = *(const float4 *)(p + (int64_t)i * 2 * kRows * 128);
+    sum.x += x.x;
+    sum.y += x.y;
+    sum.z += x.z;
+    sum.w += x.w;
+  }
+  const float mul = which ? 1.f : a.scale;
+  uint16_t *out = which ? a.dv + b * a.dvsb + h * a.dvsh + (int64_t)key * a.dvss
+                        : a.dk + b * a.dksb + h * a.dksh + (int64_t)key * a.dkss;
+  *(u32x2 *)(out + d) = u32x2{pack_bf16x2(sum.x * mul, sum.y * mul), pack_bf16x2(sum.z * mul, sum.w * mul)};
+}
+
+// Tiles that hold first keys, and the runs each is cut into: as many as make a run no
+// longer than a window tile's.
+static void plan_dkdv(WindowArgs &a) {
+  const int64_t range = (int64_t)kRows + a.left + a.right;
+  a.nkt = (a.Skv + kRows - 1) / kRows;
+  a.first_tiles = (a.sinks + kRows - 1) / kRows;
+  a.pieces = (int)((a.Sq + range - 1) / range);
+  if (a.first_tiles == 0 || a.pieces == 1) a.first_tiles = 0, a.pieces = 1;
+}
+
+size_t window_bwd_bytes(WindowArgs a) {
+  plan_dkdv(a);
+  const size_t delta = ((size_t)a.B * a.H * a.Sq * sizeof(float) + 255) / 256 * 256;
+  return delta + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
 }
 
 int launch_window_fwd(WindowArgs a, hipStream_t s) {
@@ -462,16 +536,22 @@ int launch_window_fwd(WindowArgs a, hipStream_t s) {
   return check_launch("window_fwd_kernel");
 }
 
-int launch_window_bwd(WindowArgs a, hipStream_t s) {
+int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {
+  a.delta = static_cast<float *>(ws);
   a.nqt = (a.Sq + kRows - 1) / kRows;
   a.total = a.B * a.H * a.nqt;
   hipLaunchKernelGGL(window_dq_kernel, dim3((unsigned)a.total), dim3(256), 0, s, a);
   int rc = check_launch("window_dq_kernel");
   if (rc) return rc;
-  a.nkt = (a.Skv + kRows - 1) / kRows;
-  a.total = a.B * a.Hkv * a.nkt;
+  plan_dkdv(a);
+  a.part = a.delta + ((size_t)a.B * a.H * a.Sq + 63) / 64 * 64;
+  a.total = a.B * a.Hkv * (a.nkt + a.first_tiles * (a.pieces - 1));
   hipLaunchKernelGGL(window_dkdv_kernel, dim3((unsigned)a.total), dim3(256), 0, s, a);
-  return check_launch("window_dkdv_kernel");
+  rc = check_launch("window_dkdv_kernel");
+  if (rc || a.first_tiles == 0) return rc;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.first_tiles * kRows * 2;
+  hipLaunchKernelGGL(window_dkdv_sum_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
+  return check_launch("window_dkdv_sum_kernel");
 }
 
 }  // namespace h3a

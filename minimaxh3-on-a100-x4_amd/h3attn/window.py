@@ -143,7 +143,7 @@ def attn_bwd_window(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     with _on_device(q):
         n = ctypes.c_size_t(0)
         check("h3a_attn_bwd_window_workspace_size",
-              lib().h3a_attn_bwd_window_workspace_size(B, H, Hkv, Sq, Skv, D, ctypes.byref(n)))
+              lib().h3a_attn_bwd_window_workspace_size(B, H, Hkv, Sq, Skv, D, ctypes.byref(w), ctypes.byref(n)))
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
         rc = lib().h3a_attn_bwd_window(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                        lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Sq,

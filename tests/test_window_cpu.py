@@ -48,9 +48,12 @@ def test_forward_refusals():
 def test_backward_refusals():
     L = _lib.lib()
     n = ctypes.c_size_t(0)
-    assert L.h3a_attn_bwd_window_workspace_size(1, 2, 1, 4, 4, 128, None) == _lib.H3A_ERR_INVALID_ARG
-    assert L.h3a_attn_bwd_window_workspace_size(1, 2, 1, 4, 4, 64, ctypes.byref(n)) == _lib.H3A_ERR_UNSUPPORTED
-    assert L.h3a_attn_bwd_window_workspace_size(1, 2, 1, 4, 4, 128, ctypes.byref(n)) == 0 and n.value > 0
+    w = ctypes.byref(_lib.Window(3, 3, 1, 0, 0, None, None))
+    size = L.h3a_attn_bwd_window_workspace_size
+    assert size(1, 2, 1, 4, 4, 128, w, None) == _lib.H3A_ERR_INVALID_ARG
+    assert size(1, 2, 1, 4, 4, 128, None, ctypes.byref(n)) == _lib.H3A_ERR_INVALID_ARG
+    assert size(1, 2, 1, 4, 4, 64, w, ctypes.byref(n)) == _lib.H3A_ERR_UNSUPPORTED
+    assert size(1, 2, 1, 4, 4, 128, w, ctypes.byref(n)) == 0 and n.value > 0
 
     def bwd(ptrs=(16,) * 9, st=(ROW,) * 8, ws=16, nbytes=n.value):
         win = _lib.Window(3, 3, 1, 0, 0, None, None)
