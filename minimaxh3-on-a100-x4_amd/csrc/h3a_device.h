@@ -97,6 +97,11 @@ __device__ __forceinline__ void buffer_load_lds_b128(u32x4 desc, uint32_t byte_o
                : "memory");
 }
 
+// The same for 4 bytes per lane: to lds_dst + 4 * lane.
+__device__ __forceinline__ void buffer_load_lds_b32(u32x4 desc, uint32_t byte_off, uint32_t m0) {
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(byte_off), "s"(desc), "{m0}"(m0) : "memory");
+}
+
 // The same from a 64-bit address per lane, with no range check.
 __device__ __forceinline__ void global_load_lds_b128(const void *p, uint32_t m0) {
   asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(m0) : "memory");
@@ -127,6 +132,14 @@ __device__ __forceinline__ u32x4 stage_desc(const uint16_t *base, int64_t stride
   return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
                (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xffffu)),
                (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufferConfig};
+}
+
+// The V# of `bytes` bytes from p (wave-uniform).
+__device__ __forceinline__ u32x4 range_desc(const void *p, int bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(p);
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xffffu)),
+               (uint32_t)__builtin_amdgcn_readfirstlane(bytes), (uint32_t)kBufferConfig};
 }
 
 // s_waitcnt vmcnt(N): at most the N most recent vector-memory loads of this

@@ -133,7 +133,7 @@ struct WindowArgs {
   const int32_t *q_starts, *kv_lens;  // per sequence, or null
   float scale, sl2;                   // softmax scale, and times log2(e)
   int nqt, nkt;  // 128-row query and key tiles per head
-  int total;     // workgroups
+  int chunk;     // consecutive tiles of a head on one XCD
   // backward only
   const uint16_t *dout;
   uint16_t *dq, *dk, *dv;
@@ -141,7 +141,9 @@ struct WindowArgs {
   int64_t dqsb, dqsh, dqss;
   int64_t dksb, dksh, dkss;
   int64_t dvsb, dvsh, dvss;
-  float *delta;  // [B,H,Sq] dO.O
+  float *stats;     // [2][stats_n]: lse in log2 units and dO.O of every row [B,H,Sq]
+  int64_t stats_n;
+  int grid_whole, grid_pieces, chunk_pieces;  // workgroups of dK (and of dV) for whole key tiles and for pieces
   int first_tiles, pieces;  // key tiles cut into runs of queries, and the runs of each
   float *part;              // their partial sums: [B,Hkv,first_tiles,pieces][dK, dV][128][128]
 };

@@ -15,7 +15,6 @@
 // the dense kernel rounds P); scores, softmax statistics and all sums are fp32.
 #include "h3a_device.h"
 #include "h3a_internal.h"
-#include "h3a_queue.h"
 #include "h3a_tile.h"
 
 namespace h3a {
@@ -178,14 +177,21 @@ __device__ __forceinline__ void mask_band(f32x16 (&s)[2], int key0, int g, int l
     }
 }
 
-// Work item -> (tile, head, batch), consecutive tiles of a head on one XCD.
+// Work items: `tiles` per head, dealt to the XCDs in runs of `chunk` consecutive ones, so
+// that neighbours, which read nearly the same keys, share an L2.  Workgroup i runs on
+// XCD i % 8; which of a round's 8 runs an XCD gets is rotated by a hash of the round, so
+// that no XCD is left with all the short ends of a padded batch, whatever the number of
+// runs per head (B=2 H=56/8 S=8192, one sequence less than half as long: forward 1.03 ->
+// 0.77 ms against one contiguous range per XCD).
 struct Item {
-  int tile, h, b;
+  int tile, h, b;  // tile < 0: none
 };
-__device__ __forceinline__ Item item_of(int total, int tiles, int heads) {
-  const int w = xcd_remap((int)blockIdx.x, total);
-  const int bh = w / tiles;
-  return {w % tiles, bh % heads, bh / heads};
+__device__ __forceinline__ Item item_of(const WindowArgs &a, int i, int chunk, int tiles, int heads) {
+  const int x = i & 7, k = i >> 3;
+  const int n = k / chunk, run = n * 8 + ((x + (int)((uint32_t)n * 2654435761u >> 29)) & 7);
+  const int runs = (tiles + chunk - 1) / chunk, bh = run / runs;
+  const int tile = (run % runs) * chunk + k % chunk;
+  return {bh < a.B * heads && tile < tiles ? tile : -1, bh % heads, bh / heads};
 }
 
 // Forward.  A workgroup takes 128 query rows of one head, a wave 32 of them; the
@@ -196,7 +202,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][StageBytes<L>::kK / 2], vbuf[2][StageBytes<L>::kV / 2];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Item it = item_of(a.total, a.nqt, a.H);
+  const Item it = item_of(a, (int)blockIdx.x, a.chunk, a.nqt, a.H);
+  if (it.tile < 0) return;
   const Span sp = span_of(a, it.b);
   const int q0 = it.tile * kRows, wq0 = q0 + 32 * wave, row = wq0 + l32;
   const int r0 = q0 > sp.i_lo ? q0 : sp.i_lo, r1 = (q0 + kRows < sp.i_hi ? q0 + kRows : sp.i_hi) - 1;
@@ -254,14 +261,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
                   a.o + it.b * a.osb + it.h * a.osh + (int64_t)wq0 * a.oss, a.oss, a.Sq - wq0, lane);
 }
 
-// Backward, dQ: tiles and stages as forward, with P from the stored lse.  The tile's
-// delta = dO.O goes to a.delta for the second kernel.
+// Backward, dQ: tiles and stages as forward, with P from the stored lse.  The rows' lse
+// (log2 units; +inf, so that p = 0, for a row that saw nothing) and delta = dO.O go to
+// a.stats for the second kernel.
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dq_kernel(WindowArgs a) {
   using L = DualLayout;
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][StageBytes<L>::kK / 2], vbuf[2][StageBytes<L>::kK / 2];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Item it = item_of(a.total, a.nqt, a.H);
+  const Item it = item_of(a, (int)blockIdx.x, a.chunk, a.nqt, a.H);
+  if (it.tile < 0) return;
   const Span sp = span_of(a, it.b);
   const int q0 = it.tile * kRows, wq0 = q0 + 32 * wave, row = wq0 + l32;
   const int r0 = q0 > sp.i_lo ? q0 : sp.i_lo, r1 = (q0 + kRows < sp.i_hi ? q0 + kRows : sp.i_hi) - 1;
@@ -302,9 +311,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       delta = half_swap_sum(delta);
     }
     const int64_t stat = ((int64_t)it.b * a.H + it.h) * a.Sq + (row < a.Sq ? row : a.Sq - 1);
-    if (g == 0 && row < a.Sq) a.delta[stat] = delta;
-    // A row without a finite lse saw nothing: p = exp2(-inf) = 0.
     const float l2 = a.lse[stat] == kNegInf ? -kNegInf : a.lse[stat] * kLog2e;
+    if (g == 0 && row < a.Sq) {
+      a.stats[stat] = l2;
+      a.stats[a.stats_n + stat] = delta;
+    }
     const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
     wait_vmem_all();
     __syncthreads();
@@ -335,37 +346,40 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
                   a.dq + it.b * a.dqsb + it.h * a.dqsh + (int64_t)wq0 * a.dqss, a.dqss, a.Sq - wq0, lane);
 }
 
-// Backward, dK and dV: a workgroup takes 128 keys of one key head, a wave 32 of them as
-// columns, and streams the queries that see them, of every head that shares the keys,
-// in 64-row stages of Q and dO.  A key's queries are one interval of positions, so the
-// sums run in a fixed order with no atomics.
+// Backward, dK and dV: a workgroup sums one of them over 128 keys of one key head, a wave
+// 32 of them as columns, and streams the queries that see them, of every head that
+// shares the keys, in 64-row stages of Q and dO.  A key's queries are one interval of
+// positions, so the sums run in a fixed order with no atomics.
+//
+// Both sums take the scores: 5 products for the 4 of one workgroup taking both.  But a
+// wave's 192 registers of K, V and two sums leave nothing to read LDS ahead with (two
+// waves per SIMD wait for every operand and spill: 2.7 ms at B=2 H=56/8 S=8192 with 1024
+// keys to either side); alone on its SIMD it moves scores between register files for as
+// long as it multiplies (3.5 ms); and waves of both kinds in one workgroup run their
+// softmax at the same time (2.9 ms).
 //
 // The first keys are seen by every query, the others by a window's: tiles that hold
 // first keys are cut into a.pieces equal runs of stages, which leave fp32 partial sums
-// in a.part for window_dkdv_sum_kernel.
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dkdv_kernel(WindowArgs a) {
+// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being the shortest,
+// and dK before dV.
+constexpr int kQStage = 64;
+struct DkdvLds {
+  uint16_t q[2][kQStage * 128], dout[2][kQStage * 128];
+  float stats[2][2][kQStage];  // lse (log2 units), delta
+};
+
+template <bool kDk>
+__device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item &it, int piece, DkdvLds &lds) {
   using L = DualLayout;
-  constexpr int kQ = 64;  // queries per stage
-  __shared__ __attribute__((aligned(16))) uint16_t qbuf[2][kQ * 128], dbuf[2][kQ * 128];
-  __shared__ __attribute__((aligned(16))) float stats[2][2][kQ];  // lse (log2 units), delta
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int first_items = a.first_tiles * a.pieces, per_bh = a.nkt - a.first_tiles + first_items;
-  Item it = item_of(a.total, per_bh, a.Hkv);
-  int piece = -1;  // of tile it.tile
-  if (it.tile < first_items) {
-    piece = it.tile % a.pieces;
-    it.tile /= a.pieces;
-  } else {
-    it.tile -= first_items - a.first_tiles;
-  }
   const Span sp = span_of(a, it.b);
   const int j0 = it.tile * kRows, wj0 = j0 + 32 * wave, key = wj0 + l32;
   const int j1 = (j0 + kRows < sp.len ? j0 + kRows : sp.len) - 1;
 
-  f32x16 dk[4], dv[4];
+  f32x16 acc[4];
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt) dk[dt] = dv[dt] = f32x16{0.f};
+  for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{0.f};
   // Rows [i_a, i_b) see some key of the tile.
   int i_a = sp.i_lo, i_b = sp.i_hi;
   if (j0 >= a.sinks) {
@@ -374,118 +388,152 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   } else if (a.causal) {
     i_a = j0 - sp.qs > i_a ? j0 - sp.qs : i_a;
   }
-  // Stage t: rows i0 .. of head h; stages t_a .. t_b - 1 are this piece's.
-  const int per_head = j1 >= j0 && i_b > i_a ? (i_b - i_a + kQ - 1) / kQ : 0;
+  // Stages t_a .. t_a + n - 1 are this piece's: kQStage rows of a head, head after head.
+  const int per_head = j1 >= j0 && i_b > i_a ? (i_b - i_a + kQStage - 1) / kQStage : 0;
   const int64_t stages = (int64_t)per_head * a.rep;
   const int64_t t_a = piece < 0 ? 0 : stages * piece / a.pieces;
-  const int64_t t_b = piece < 0 ? stages : stages * (piece + 1) / a.pieces;
-  if (t_b > t_a) {
-    // Positions that see the lane's key.
-    int plo = key - a.right, phi = key + a.left;
+  const int n = (int)((piece < 0 ? stages : stages * (piece + 1) / a.pieces) - t_a);
+  if (n > 0) {
+    // Positions plo .. plo + span see the lane's key.
+    int plo = key - a.right;
+    uint32_t span = (uint32_t)(a.left + a.right);
     if (key < a.sinks) {
       plo = a.causal ? key : -(1 << 30);
-      phi = 1 << 30;
+      span = 0x7fffffffu;
     }
-    if (key >= sp.len) phi = -(1 << 30), plo = 1 << 30;
-    const bool keys_whole = wj0 + 31 < sp.len;
-    u32x4 kf[8], vf[8];
-    load_columns(kf, a.k + it.b * a.ksb + it.h * a.ksh, a.kss, key, sp.len, g);
-    load_columns(vf, a.v + it.b * a.vsb + it.h * a.vsh, a.vss, key, sp.len, g);
-    TileDma<4, L, false, kQ> qdma, ddma;
+    if (key >= sp.len) plo = 1 << 30, span = 0;
+    TileDma<4, L, false, kQStage> qdma, ddma;
     qdma.init(a.qss, wave, lane);
     ddma.init(a.gss, wave, lane);
-    int h = it.h * a.rep + (int)(t_a / per_head), i0 = i_a + (int)(t_a % per_head) * kQ;
-    float st_next = 0.f;
-    auto fetch = [&](int buf) __attribute__((always_inline)) {
-      qdma.issue(a.q + it.b * a.qsb + h * a.qsh, a.qss, i0, i_b, qbuf[buf]);
-      ddma.issue(a.dout + it.b * a.gsb + h * a.gsh, a.gss, i0, i_b, dbuf[buf]);
-      // Waves 0 and 1 take the rows' lse and delta; rows past the end get p = 0.
-      if (wave < 2) {
-        const int i = i0 + lane;
-        const int64_t at = ((int64_t)it.b * a.H + h) * a.Sq + (i < i_b ? i : i_b - 1);
-        const float x = wave == 0 ? a.lse[at] : a.delta[at];
-        if (wave == 0) st_next = i < i_b && x != kNegInf ? x * kLog2e : -kNegInf;
-        else st_next = i < i_b ? x : 0.f;
+    int fh = it.h * a.rep + (int)(t_a / per_head), frow = i_a + (int)(t_a % per_head) * kQStage;
+    int crow = frow;  // rows of the stage that is computed
+    auto fetch = [&](int slot) __attribute__((always_inline)) {
+      qdma.issue(a.q + it.b * a.qsb + fh * a.qsh, a.qss, frow, i_b, lds.q[slot]);
+      ddma.issue(a.dout + it.b * a.gsb + fh * a.gsh, a.gss, frow, i_b, lds.dout[slot]);
+      // Rows past i_b are zeros throughout: p = 1, but dO = dP = delta = 0.
+      if (wave < (kDk ? 2 : 1)) {
+        const int rows = i_b - frow < kQStage ? i_b - frow : kQStage;
+        const float *st = a.stats + wave * a.stats_n + ((int64_t)it.b * a.H + fh) * a.Sq + frow;
+        buffer_load_lds_b32(range_desc(st, rows * 4), 4 * lane, lds_address(lds.stats[slot][wave]));
+      }
+      frow += kQStage;
+      if (frow >= i_b) {
+        frow = i_a;
+        ++fh;
       }
     };
     fetch(0);
-    if (wave < 2) stats[0][wave][lane] = st_next;
+    u32x4 kf[8], vf[kDk ? 8 : 1];
+    load_columns(kf, a.k + it.b * a.ksb + it.h * a.ksh, a.kss, key, sp.len, g);
+    if constexpr (kDk) load_columns(vf, a.v + it.b * a.vsb + it.h * a.vsh, a.vss, key, sp.len, g);
     const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
+    const bool keys_whole = wj0 + 31 < sp.len;
+    // What the wave's keys are to rows at positions p0 .. p0 + 63 (those past i_b give
+    // nothing whatever p is).
+    auto cover = [&](int p0) __attribute__((always_inline)) -> Cover {
+      const int p1 = p0 + kQStage - 1;
+      if (wj0 >= sp.len) return kNone;
+      if (wj0 < a.sinks) {
+        if (a.causal && p1 < wj0) return kNone;
+        if (wj0 + 31 < a.sinks) return keys_whole && (!a.causal || p0 >= wj0 + 31) ? kAll : kPart;
+      } else if (p1 < wj0 - a.right || p0 > wj0 + 31 + a.left) {
+        return kNone;
+      }
+      return keys_whole && p0 >= wj0 + 31 - a.right && p1 <= (wj0 < a.sinks ? a.sinks : wj0) + a.left ? kAll : kPart;
+    };
+    // Row statistics of accumulator registers 4*r4 .. 4*r4+3 of sub-tile u.
+    auto row_stats = [&](int slot, int which, int u, int r4, float(&x)[4]) __attribute__((always_inline)) {
+      const float4 v = *(const float4 *)&lds.stats[slot][which][32 * u + 8 * r4 + 4 * g];
+      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    };
     wait_vmem_all();
     __syncthreads();
-    const int total = (int)(t_b - t_a);
-    for (int t = 0; t < total; ++t) {
-      const int buf = t & 1, p_stage = sp.qs + i0, rows = i_b - i0;
-      i0 += kQ;
-      if (i0 >= i_b) {
-        i0 = i_a;
-        ++h;
-      }
-      if (t + 1 < total) fetch(buf ^ 1);
-#pragma unroll 1  // one 32-row half's registers at a time
-      for (int u = 0; u < kQ / 32; ++u) {
-        const int p0 = p_stage + 32 * u, p1 = p0 + 31;
-        bool none = rows <= 32 * u, all = keys_whole && rows >= 32 * u + 32;
-        if (wj0 < a.sinks) {
-          none = none || (a.causal && p1 < wj0);
-          if (wj0 + 31 >= a.sinks) all = all && p0 >= wj0 + 31 - a.right && p1 <= a.sinks + a.left;
-          else all = all && (!a.causal || p0 >= wj0 + 31);
-        } else {
-          none = none || p1 < wj0 - a.right || p0 > wj0 + 31 + a.left;
-          all = all && p0 >= wj0 + 31 - a.right && p1 <= wj0 + a.left;
-        }
-        if (none) continue;
-        const uint16_t *qt = qbuf[buf] + u * 32 * 128, *dt = dbuf[buf] + u * 32 * 128;
-        f32x16 s[1], dp[1];
-        u32x4 pf[2], dsf[2];
-        score_tile<L, 1>(qt, kf, k_rd, s);
-        score_tile<L, 1>(dt, vf, k_rd, dp);
+    for (int j = 0; j < n; ++j) {
+      const int slot = j & 1, p0 = sp.qs + crow;
+      crow += kQStage;
+      if (crow >= i_b) crow = i_a;
+      if (j + 1 < n) fetch(slot ^ 1);
+      const Cover c = cover(p0);
+      if (c != kNone) {
+        f32x16 s[2];
+        u32x4 f[4];
+        score_tile<L, 2>(lds.q[slot], kf, k_rd, s);
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const float4 l2 = *(const float4 *)&stats[buf][0][32 * u + 8 * r4 + 4 * g];
-          const float4 de = *(const float4 *)&stats[buf][1][32 * u + 8 * r4 + 4 * g];
-          const float lv[4] = {l2.x, l2.y, l2.z, l2.w}, dl[4] = {de.x, de.y, de.z, de.w};
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int pos = p0 + 8 * r4 + 4 * g + r;
-            float p = fast_exp2(fmaf(s[0][4 * r4 + r], a.sl2, -lv[r]));
-            float ds = p * (dp[0][4 * r4 + r] - dl[r]);
-            if (!all && !(pos >= plo && pos <= phi)) p = ds = 0.f;
-            s[0][4 * r4 + r] = p;
-            dp[0][4 * r4 + r] = ds;
+          for (int r4 = 0; r4 < 4; ++r4) {
+            float l2[4];
+            row_stats(slot, 0, u, r4, l2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[u][4 * r4 + r] = fast_exp2(fmaf(s[u][4 * r4 + r], a.sl2, -l2[r]));
           }
+        if constexpr (kDk) {
+          f32x16 dp[2];
+          score_tile<L, 2>(lds.dout[slot], vf, k_rd, dp);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+              float de[4];
+              row_stats(slot, 1, u, r4, de);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[u][4 * r4 + r] *= dp[u][4 * r4 + r] - de[r];
+            }
         }
-        pack_p<1>(s, pf);
-        pack_p<1>(dp, dsf);
-        transposed_product<2>(dt, pf, t_rd, dv);
-        transposed_product<2>(qt, dsf, t_rd, dk);
+        if (c == kPart) {  // p or ds of rows that do not see the key
+          const uint32_t ahead = (uint32_t)(p0 + 4 * g - plo);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (ahead + 32 * u + 8 * (r >> 2) + (r & 3) > span) s[u][r] = 0.f;
+        }
+        pack_p<2>(s, f);
+        transposed_product<4>(kDk ? lds.q[slot] : lds.dout[slot], f, t_rd, acc);
       }
-      if (t + 1 < total && wave < 2) stats[buf ^ 1][wave][lane] = st_next;
       wait_vmem_all();
       __syncthreads();
     }
   }
   if (piece >= 0) {
     const int64_t bh = (int64_t)it.b * a.Hkv + it.h;
-    float *part = a.part + ((bh * a.first_tiles + it.tile) * a.pieces + piece) * (2 * kRows * 128) +
+    float *part = a.part + (((bh * a.first_tiles + it.tile) * a.pieces + piece) * 2 + (kDk ? 0 : 1)) * (kRows * 128) +
                   (32 * wave + l32) * 128 + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int rr = 0; rr < 4; ++rr) {
+      for (int rr = 0; rr < 4; ++rr)
         *(float4 *)(part + dt * 32 + 8 * rr) =
-            float4{dk[dt][4 * rr], dk[dt][4 * rr + 1], dk[dt][4 * rr + 2], dk[dt][4 * rr + 3]};
-        *(float4 *)(part + kRows * 128 + dt * 32 + 8 * rr) =
-            float4{dv[dt][4 * rr], dv[dt][4 * rr + 1], dv[dt][4 * rr + 2], dv[dt][4 * rr + 3]};
-      }
+            float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]};
   } else if (wj0 < a.Skv) {
-    const bool live = key < sp.len;
-    uint8_t *tile = reinterpret_cast<uint8_t *>(&qbuf[0][0]) + wave * 8192;
-    store_columns(dk, a.scale, live, tile, a.dk + it.b * a.dksb + it.h * a.dksh + (int64_t)wj0 * a.dkss, a.dkss,
-                  a.Skv - wj0, lane);
-    store_columns(dv, 1.f, live, tile, a.dv + it.b * a.dvsb + it.h * a.dvsh + (int64_t)wj0 * a.dvss, a.dvss,
-                  a.Skv - wj0, lane);
+    uint8_t *tile = reinterpret_cast<uint8_t *>(&lds.q[0][0]) + wave * 8192;
+    uint16_t *out = kDk ? a.dk + it.b * a.dksb + it.h * a.dksh + (int64_t)wj0 * a.dkss
+                        : a.dv + it.b * a.dvsb + it.h * a.dvsh + (int64_t)wj0 * a.dvss;
+    store_columns(acc, kDk ? a.scale : 1.f, key < sp.len, tile, out, kDk ? a.dkss : a.dvss, a.Skv - wj0, lane);
   }
+}
+
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dkdv_kernel(WindowArgs a) {
+  __shared__ __attribute__((aligned(16))) DkdvLds lds;
+  // The grid: dK and dV of the whole tiles, then dK and dV of the pieces.
+  int i = (int)blockIdx.x;
+  const bool whole = i < 2 * a.grid_whole;
+  if (!whole) i -= 2 * a.grid_whole;
+  const int half = whole ? a.grid_whole : a.grid_pieces;
+  const bool dv = i >= half;
+  if (dv) i -= half;
+  Item it = whole ? item_of(a, i, a.chunk, a.nkt - a.first_tiles, a.Hkv)
+                  : item_of(a, i, a.chunk_pieces, a.first_tiles * a.pieces, a.Hkv);
+  if (it.tile < 0) return;
+  int piece = -1;  // of tile it.tile
+  if (whole) {
+    it.tile += a.first_tiles;
+  } else {
+    piece = it.tile % a.pieces;
+    it.tile /= a.pieces;
+  }
+  if (dv) window_key_sums<false>(a, it, piece, lds);
+  else window_key_sums<true>(a, it, piece, lds);
 }
 
 // dK and dV of the tiles that were cut: the pieces' partial sums in order.  A thread
@@ -520,33 +568,48 @@ static void plan_dkdv(WindowArgs &a) {
   a.nkt = (a.Skv + kRows - 1) / kRows;
   a.first_tiles = (a.sinks + kRows - 1) / kRows;
   a.pieces = (int)((a.Sq + range - 1) / range);
-  if (a.first_tiles == 0 || a.pieces == 1) a.first_tiles = 0, a.pieces = 1;
+  if (a.first_tiles == 0 || a.pieces == 1) {
+    a.first_tiles = 0;
+    a.pieces = 1;
+  }
 }
+
+// Rows of each of the two statistics, padded to 256 bytes.
+static size_t stat_rows(const WindowArgs &a) { return ((size_t)a.B * a.H * a.Sq + 63) / 64 * 64; }
 
 size_t window_bwd_bytes(WindowArgs a) {
   plan_dkdv(a);
-  const size_t delta = ((size_t)a.B * a.H * a.Sq * sizeof(float) + 255) / 256 * 256;
-  return delta + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
+  return 2 * stat_rows(a) * sizeof(float) + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
+}
+
+// Grid of `tiles` work items for each of `heads` heads (item_of).
+static int deal(int tiles, int heads, int *chunk) {
+  const int64_t total = (int64_t)heads * tiles;
+  *chunk = total / 512 < 1 ? 1 : (total / 512 > 16 ? 16 : (int)(total / 512));
+  const int64_t runs = (int64_t)heads * ((tiles + *chunk - 1) / *chunk);
+  return (int)((runs + 7) / 8 * 8 * *chunk);
 }
 
 int launch_window_fwd(WindowArgs a, hipStream_t s) {
   a.nqt = (a.Sq + kRows - 1) / kRows;
-  a.total = a.B * a.H * a.nqt;
-  hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)a.total), dim3(256), 0, s, a);
+  const int grid = deal(a.nqt, a.B * a.H, &a.chunk);
+  hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   return check_launch("window_fwd_kernel");
 }
 
 int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {
-  a.delta = static_cast<float *>(ws);
+  a.stats = static_cast<float *>(ws);
+  a.stats_n = (int64_t)stat_rows(a);
   a.nqt = (a.Sq + kRows - 1) / kRows;
-  a.total = a.B * a.H * a.nqt;
-  hipLaunchKernelGGL(window_dq_kernel, dim3((unsigned)a.total), dim3(256), 0, s, a);
+  const int grid = deal(a.nqt, a.B * a.H, &a.chunk);
+  hipLaunchKernelGGL(window_dq_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   int rc = check_launch("window_dq_kernel");
   if (rc) return rc;
   plan_dkdv(a);
-  a.part = a.delta + ((size_t)a.B * a.H * a.Sq + 63) / 64 * 64;
-  a.total = a.B * a.Hkv * (a.nkt + a.first_tiles * (a.pieces - 1));
-  hipLaunchKernelGGL(window_dkdv_kernel, dim3((unsigned)a.total), dim3(256), 0, s, a);
+  a.part = a.stats + 2 * a.stats_n;
+  a.grid_whole = deal(a.nkt - a.first_tiles, a.B * a.Hkv, &a.chunk);
+  a.grid_pieces = deal(a.first_tiles * a.pieces, a.B * a.Hkv, &a.chunk_pieces);
+  hipLaunchKernelGGL(window_dkdv_kernel, dim3((unsigned)(2 * a.grid_whole + 2 * a.grid_pieces)), dim3(256), 0, s, a);
   rc = check_launch("window_dkdv_kernel");
   if (rc || a.first_tiles == 0) return rc;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.first_tiles * kRows * 2;
