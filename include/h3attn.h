@@ -247,13 +247,18 @@ typedef struct {
  * Forward.  lse [B,H,Sq] fp32 contiguous (may be NULL): log of the sum of
  * exp(scale * q.k) over the keys seen, for h3a_attn_bwd_window.  Strides and
  * alignment as h3a_attn_fwd, and every sequence stride < 2^24 elements; lengths
- * up to 2^29.  No counterpart in the reference.
+ * up to 2^29.  workspace: h3a_attn_fwd_window_workspace_size bytes for the current
+ * device (0, so NULL, for more than 256 rows: fewer may be split along the keys),
+ * untouched until the call's work has completed.  No counterpart in the reference.
  */
+int h3a_attn_fwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D,
+                                       const h3a_window *window, size_t *bytes);
 int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, float *lse,
                         int B, int H, int Hkv, int Sq, int Skv, int D,
                         const int64_t q_strides[3], const int64_t k_strides[3],
                         const int64_t v_strides[3], const int64_t o_strides[3],
-                        const h3a_window *window, float scale, h3a_stream_t stream);
+                        const h3a_window *window, float scale, void *workspace, size_t workspace_bytes,
+                        h3a_stream_t stream);
 
 /*
  * Backward: dq, dk, dv (bf16, in the shapes of q, k, v) from dout (bf16, as o) and

@@ -560,10 +560,22 @@ int h3a_attn_fwd_blocksparse_tiles_ws(const void *q, const void *k, const void *
   return launch_attn_sparse_split(a, 64, plan, workspace, as_stream(stream), true);
 }
 
+int h3a_attn_fwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, const h3a_window *window,
+                                       size_t *bytes) {
+  clear_error();
+  if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
+  int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
+  if (!rc) rc = check_window(window, Sq, Skv, 1.f);
+  if (rc) return rc;
+  WindowArgs a;
+  fill_window_args(a, B, H, Hkv, Sq, Skv, *window, 1.f);
+  return window_fwd_bytes(a, bytes);
+}
+
 int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, float *lse, int B, int H, int Hkv,
                         int Sq, int Skv, int D, const int64_t q_strides[3], const int64_t k_strides[3],
                         const int64_t v_strides[3], const int64_t o_strides[3], const h3a_window *window,
-                        float scale, h3a_stream_t stream) {
+                        float scale, void *workspace, size_t workspace_bytes, h3a_stream_t stream) {
   clear_error();
   int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
   if (!rc) rc = check_window(window, Sq, Skv, scale);
@@ -584,7 +596,13 @@ int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, fl
   put_strides(a.ksb, a.ksh, a.kss, k_strides, Skv);
   put_strides(a.vsb, a.vsh, a.vss, v_strides, Skv);
   put_strides(a.osb, a.osh, a.oss, o_strides, Sq);
-  return launch_window_fwd(a, as_stream(stream));
+  size_t need = 0;
+  rc = window_fwd_bytes(a, &need);
+  if (rc) return rc;
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(H3A_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+  if (need > 0 && !aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  return launch_window_fwd(a, workspace, as_stream(stream));
 }
 
 int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, const h3a_window *window,

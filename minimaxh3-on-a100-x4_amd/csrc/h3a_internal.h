@@ -147,7 +147,8 @@ struct WindowArgs {
   int first_tiles, pieces;  // key tiles cut into runs of queries, and the runs of each
   float *part;              // their partial sums: [B,Hkv,first_tiles,pieces][dK, dV][128][128]
 };
-int launch_window_fwd(WindowArgs a, hipStream_t s);
+int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s);
+int window_fwd_bytes(WindowArgs a, size_t *bytes);  // workspace on the current device
 int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s);
 size_t window_bwd_bytes(WindowArgs a);  // workspace, from the sizes and the window
 

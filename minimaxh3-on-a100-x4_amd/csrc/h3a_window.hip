@@ -129,6 +129,7 @@ __device__ __forceinline__ int first_keys(const WindowArgs &a, const Span &s, in
 
 // The key stages of a run of positions p0 .. p1: [0, first) and then [lo, hi), or one
 // range [0, hi) where the two meet.
+template <int BN = kBN>
 struct KeyStages {
   int n_first, n, lo, first, hi;
   __device__ __forceinline__ void init(const WindowArgs &a, const Span &s, int p0, int p1) {
@@ -140,19 +141,20 @@ struct KeyStages {
       lo = 0;
       hi = hi > first ? hi : first;
     } else {
-      n_first = (first + kBN - 1) / kBN;
+      n_first = (first + BN - 1) / BN;
     }
-    n = n_first + (hi - lo + kBN - 1) / kBN;
+    n = n_first + (hi - lo + BN - 1) / BN;
   }
-  __device__ __forceinline__ int key0(int j) const { return j < n_first ? j * kBN : lo + (j - n_first) * kBN; }
+  __device__ __forceinline__ int key0(int j) const { return j < n_first ? j * BN : lo + (j - n_first) * BN; }
   __device__ __forceinline__ int limit(int j) const { return j < n_first ? first : hi; }
 };
 
-// What a wave at positions p0 .. p1 sees of a 64-key stage: nothing, all of it, or a part.
+// What a wave at positions p0 .. p1 sees of a stage: nothing, all of it, or a part.
 enum Cover { kNone, kAll, kPart };
-__device__ __forceinline__ Cover cover_of(const WindowArgs &a, const Span &s, const KeyStages &ks, int j, int p0,
+template <int BN>
+__device__ __forceinline__ Cover cover_of(const WindowArgs &a, const Span &s, const KeyStages<BN> &ks, int j, int p0,
                                           int p1) {
-  const int k0 = ks.key0(j), k1 = k0 + kBN - 1;
+  const int k0 = ks.key0(j), k1 = k0 + BN - 1;
   const int f0 = first_keys(a, s, p0), f1 = first_keys(a, s, p1);
   if (k1 < f0) return kAll;
   if (j < ks.n_first) return k0 < f1 ? kPart : kNone;
@@ -165,11 +167,12 @@ __device__ __forceinline__ Cover cover_of(const WindowArgs &a, const Span &s, co
 
 // Scores the lane's row does not see -> `hidden`.  Keys lo .. hi and those below first
 // are seen; a stage of the first keys alone (only_first) ends at `first`.
-__device__ __forceinline__ void mask_band(f32x16 (&s)[2], int key0, int g, int lo, int hi, int first, bool only_first,
+template <int NSUB>
+__device__ __forceinline__ void mask_band(f32x16 (&s)[NSUB], int key0, int g, int lo, int hi, int first, bool only_first,
                                           float hidden) {
   const int l = only_first ? 1 << 30 : lo;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < NSUB; ++u)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = key0 + 32 * u + 8 * (r >> 2) + 4 * g + (r & 3);
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     // The wave's rows that are tokens; a wave without one takes the tile's nearest.
     auto clamp_row = [&](int i) __attribute__((always_inline)) { return i < r0 ? r0 : (i > r1 ? r1 : i); };
     const int p0 = sp.qs + clamp_row(wq0), p1 = sp.qs + clamp_row(wq0 + 31), pos = sp.qs + clamp_row(row);
-    KeyStages st;
+    KeyStages<> st;
     st.init(a, sp, sp.qs + r0, sp.qs + r1);
     const int lo = pos - a.left, first = first_keys(a, sp, pos);
     const int hi = pos + a.right < sp.len - 1 ? pos + a.right : sp.len - 1;
@@ -261,6 +264,186 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
                   a.o + it.b * a.osb + it.h * a.osh + (int64_t)wq0 * a.oss, a.oss, a.Sq - wq0, lane);
 }
 
+// Forward for few query rows (a new token, or a short chunk of them, against a cache).
+// Bound by the bytes of K and V, so the rows of all heads that share a key head ride
+// together as columns, 32 to a workgroup, and the keys are split: over a.pieces
+// workgroups, and within one over its four waves, each with its own running softmax and
+// its own double-buffered 32-key stages (no barrier until the end).  The waves merge
+// through LDS, the workgroups through a.part and window_token_sum_kernel.
+constexpr int kTokenStage = 32, kTokenRows = 32;
+struct TokenLds {
+  uint16_t k[4][2][kTokenStage * 128], v[4][2][kTokenStage * 128];  // by wave
+};
+
+// Column of a workgroup's rows -> query row and head.
+__device__ __forceinline__ int token_row(const WindowArgs &a, int col) { return col % a.Sq; }
+__device__ __forceinline__ int token_head(const WindowArgs &a, int col) { return col / a.Sq; }
+
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) window_token_kernel(WindowArgs a) {
+  using L = SwzLayout;
+  __shared__ __attribute__((aligned(16))) TokenLds lds;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int piece = (int)blockIdx.x % a.pieces, unit = (int)blockIdx.x / a.pieces;
+  const int group = unit % a.nqt, bh = unit / a.nqt, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const Span sp = span_of(a, b);
+  const int col = group * kTokenRows + l32;
+  const bool has = col < a.rep * a.Sq;
+  const int h = hk * a.rep + (has ? token_head(a, col) : 0), row = has ? token_row(a, col) : 0;
+  const int r0 = sp.i_lo, r1 = sp.i_hi - 1;
+  const bool live = has && row >= r0 && row <= r1;
+
+  f32x16 o[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) o[dt] = f32x16{0.f};
+  float m = kNegInf, lsum = 0.f;
+  if (r1 >= r0) {
+    const int p0 = sp.qs + r0, p1 = sp.qs + r1;
+    const int pos = sp.qs + (row < r0 ? r0 : (row > r1 ? r1 : row));
+    KeyStages<kTokenStage> st;
+    st.init(a, sp, p0, p1);
+    const int lo = pos - a.left, first = first_keys(a, sp, pos);
+    const int hi = pos + a.right < sp.len - 1 ? pos + a.right : sp.len - 1;
+    const int j_a = (int)((int64_t)st.n * piece / a.pieces), j_b = (int)((int64_t)st.n * (piece + 1) / a.pieces);
+    const uint16_t *Kb = a.k + b * a.ksb + hk * a.ksh, *Vb = a.v + b * a.vsb + hk * a.vsh;
+    TileDma<1, L, false, kTokenStage> kdma;
+    TileDma<1, L, true, kTokenStage> vdma;
+    kdma.init(a.kss, 0, lane);
+    vdma.init(a.vss, 0, lane);
+    constexpr int kInst = decltype(kdma)::kInst + decltype(vdma)::kInst;
+    auto fetch = [&](int j, int buf) __attribute__((always_inline)) {
+      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), lds.k[wave][buf]);
+      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), lds.v[wave][buf]);
+    };
+    int j = j_a + wave;
+    if (j < j_b) fetch(j, 0);
+    u32x4 qf[8];
+    load_columns(qf, a.q + b * a.qsb + h * a.qsh, a.qss, row, a.Sq, g);
+    const int k_rd = L::k_base(l32, g), v_rd = L::v_base(lane);
+    for (int buf = 0; j < j_b; j += 4, buf ^= 1) {
+      // The other buffer's last reads have returned; its next stage goes out before this
+      // one is waited for.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j + 4 < j_b) {
+        fetch(j + 4, buf ^ 1);
+        wait_vmem_le<kInst>();
+      } else {
+        wait_vmem_all();
+      }
+      asm volatile("" ::: "memory");
+      f32x16 s[1];
+      u32x4 pf[2];
+      score_tile<L, 1>(lds.k[wave][buf], qf, k_rd, s);
+      if (cover_of(a, sp, st, j, p0, p1) != kAll)
+        mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, kNegInf);
+      softmax_stage<1>(s, 0, kTokenStage, g, a.sl2, m, lsum, o, pf);
+      pv_tile<L, 2>(lds.v[wave][buf], pf, v_rd, o);
+    }
+  }
+  // Merge the waves: wave u takes dims 32u .. 32u+31 of all four.
+  __syncthreads();
+  float *xch = reinterpret_cast<float *>(&lds.k[0][0][0]);           // [wave][dims / 32][register][lane]
+  float2 *ml = reinterpret_cast<float2 *>(&lds.v[0][0][0]);          // [wave][lane]
+  const float ltot = half_swap_sum(lsum);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) xch[((wave * 4 + dt) * 16 + r) * 64 + lane] = o[dt][r];
+  ml[wave * 64 + lane] = float2{m, ltot};
+  __syncthreads();
+  float top = kNegInf, l = 0.f, w[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) top = fmaxf(top, ml[u * 64 + lane].x);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float2 x = ml[u * 64 + lane];
+    w[u] = x.x == kNegInf ? 0.f : fast_exp2(x.x - top);
+    l = fmaf(x.y, w[u], l);
+  }
+  const float inv = a.pieces > 1 ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+  const int64_t slot = ((int64_t)unit * a.pieces + piece) * kTokenRows + l32;
+#pragma unroll
+  for (int r4 = 0; r4 < 4; ++r4) {
+    float x[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum = fmaf(w[u], xch[((u * 4 + wave) * 16 + 4 * r4 + r) * 64 + lane], sum);
+      x[r] = live ? sum * inv : 0.f;
+    }
+    const int d = 32 * wave + 8 * r4 + 4 * g;
+    if (a.pieces > 1) *(float4 *)(a.part + slot * 128 + d) = float4{x[0], x[1], x[2], x[3]};
+    else if (has)
+      *(u32x2 *)(a.o + b * a.osb + h * a.osh + row * a.oss + d) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+  }
+  if (wave == 0 && g == 0) {
+    if (a.pieces > 1) {
+      float *stat = a.part + (int64_t)gridDim.x * kTokenRows * 128 + slot * 2;
+      *(float2 *)stat = live ? float2{top, l} : float2{kNegInf, 0.f};
+    } else if (a.lse && has) {
+      a.lse[((int64_t)b * a.H + h) * a.Sq + row] = live && l > 0.f ? (top + log2f(l)) * kLn2 : kNegInf;
+    }
+  }
+}
+
+// The pieces of a split key range: O = sum 2^(m_p - M) O_p / sum 2^(m_p - M) l_p.  A
+// workgroup takes a row: 32 lanes of 4 dims, 8 groups of them over the pieces, each with
+// all its loads in flight (28 rows of 33 pieces: 21 us as one walk per thread).
+constexpr int kTokenPieces = 64;
+__global__ void __launch_bounds__(256) window_token_sum_kernel(WindowArgs a, int units) {
+  __shared__ float4 part[8][32];
+  __shared__ float2 stat[8];
+  constexpr int kPer = kTokenPieces / 8;
+  const int unit = (int)(blockIdx.x / kTokenRows), c = (int)(blockIdx.x % kTokenRows);
+  const int grp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
+  const int group = unit % a.nqt, bh = unit / a.nqt, hk = bh % a.Hkv, b = bh / a.Hkv;
+  const int col = group * kTokenRows + c;
+  if (col >= a.rep * a.Sq) return;
+  const int h = hk * a.rep + token_head(a, col), row = token_row(a, col);
+  const float *ml = a.part + (int64_t)units * a.pieces * kTokenRows * 128;
+  const int64_t slot = (int64_t)unit * a.pieces * kTokenRows + c;
+  float2 x[kPer];
+  float4 v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int p = grp + 8 * i;
+    const int64_t at = slot + (int64_t)(p < a.pieces ? p : 0) * kTokenRows;
+    x[i] = p < a.pieces ? *(const float2 *)(ml + at * 2) : float2{kNegInf, 0.f};
+    v[i] = p < a.pieces ? *(const float4 *)(a.part + at * 128 + d) : float4{0.f, 0.f, 0.f, 0.f};
+  }
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) top = fmaxf(top, x[i].x);
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  auto add = [&](float m, float lp, const float4 &o) __attribute__((always_inline)) {
+    const float w = m == kNegInf ? 0.f : fast_exp2(m - top);
+    acc.x = fmaf(w, o.x, acc.x);
+    acc.y = fmaf(w, o.y, acc.y);
+    acc.z = fmaf(w, o.z, acc.z);
+    acc.w = fmaf(w, o.w, acc.w);
+    l = fmaf(w, lp, l);
+  };
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) add(x[i].x, x[i].y, v[i]);
+  part[grp][lane] = acc;
+  if (lane == 0) stat[grp] = float2{top, l};
+  __syncthreads();
+  if (grp != 0) return;
+  top = kNegInf;
+  acc = {0.f, 0.f, 0.f, 0.f};
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, stat[i].x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) add(stat[i].x, stat[i].y, part[i][lane]);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  *(u32x2 *)(a.o + b * a.osb + h * a.osh + row * a.oss + d) =
+      u32x2{pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv)};
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Sq + row] = l > 0.f ? (top + log2f(l)) * kLn2 : kNegInf;
+}
+
 // Backward, dQ: tiles and stages as forward, with P from the stored lse.  The rows' lse
 // (log2 units; +inf, so that p = 0, for a row that saw nothing) and delta = dO.O go to
 // a.stats for the second kernel.
@@ -284,7 +467,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   if (r1 >= r0) {
     auto clamp_row = [&](int i) __attribute__((always_inline)) { return i < r0 ? r0 : (i > r1 ? r1 : i); };
     const int p0 = sp.qs + clamp_row(wq0), p1 = sp.qs + clamp_row(wq0 + 31), pos = sp.qs + clamp_row(row);
-    KeyStages st;
+    KeyStages<> st;
     st.init(a, sp, sp.qs + r0, sp.qs + r1);
     const int lo = pos - a.left, first = first_keys(a, sp, pos);
     const int hi = pos + a.right < sp.len - 1 ? pos + a.right : sp.len - 1;
@@ -590,11 +773,69 @@ static int deal(int tiles, int heads, int *chunk) {
   return (int)((runs + 7) / 8 * 8 * *chunk);
 }
 
-int launch_window_fwd(WindowArgs a, hipStream_t s) {
-  a.nqt = (a.Sq + kRows - 1) / kRows;
-  const int grid = deal(a.nqt, a.B * a.H, &a.chunk);
-  hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
-  return check_launch("window_fwd_kernel");
+// Query rows up to which splitting the keys is weighed against the tiles.
+constexpr int kTokenMaxRows = 256;
+
+// Whether the keys are split, and into how many workgroups per 32 rows.  In units of a
+// token workgroup's step (four waves' stages of 32 keys, about 2 us of its CU): a round of
+// workgroups costs three steps beside its own, the merge four, and a 64-key stage of the
+// tiles 0.7 (two workgroups to a CU).
+static bool plan_token(WindowArgs &a, int cus) {
+  if (a.Sq > kTokenMaxRows) return false;
+  a.nqt = (a.rep * a.Sq + kTokenRows - 1) / kTokenRows;
+  const int64_t units = (int64_t)a.B * a.Hkv * a.nqt;
+  const int64_t range = (int64_t)a.left + a.right + a.Sq < a.Skv ? (int64_t)a.left + a.right + a.Sq : a.Skv;
+  const int64_t keys = range + a.sinks < a.Skv ? range + a.sinks : a.Skv;
+  const int64_t steps = (keys + 4 * kTokenStage - 1) / (4 * kTokenStage);
+  const int64_t tiles = (int64_t)a.B * a.H * ((a.Sq + kRows - 1) / kRows);
+  int64_t best = (tiles + 2 * cus - 1) / (2 * cus) * ((keys + kBN - 1) / kBN) * 7 / 10 + 3;
+  a.pieces = 0;
+  for (int p = 1; p <= kTokenPieces && p <= steps; ++p) {
+    const int64_t rounds = (units * p + cus - 1) / cus;
+    const int64_t cost = rounds * ((steps + p - 1) / p + 3) + (p > 1 ? 4 : 0);
+    if (cost < best || (p == 1 && a.Sq == 1)) {  // (a lone row never takes a tile)
+      best = cost;
+      a.pieces = p;
+    }
+  }
+  return a.pieces > 0;
+}
+
+static int cu_count(int *cus) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || *cus <= 0)
+    return fail(H3A_ERR_HIP, "device query failed");
+  return H3A_OK;
+}
+
+int window_fwd_bytes(WindowArgs a, size_t *bytes) {
+  *bytes = 0;
+  if (a.Sq > kTokenMaxRows) return H3A_OK;
+  int cus = 0;
+  const int rc = cu_count(&cus);
+  if (rc) return rc;
+  if (plan_token(a, cus) && a.pieces > 1) *bytes = (size_t)a.B * a.Hkv * a.nqt * a.pieces * kTokenRows * (128 + 2) * sizeof(float);
+  return H3A_OK;
+}
+
+int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
+  int cus = 0;
+  int rc = a.Sq <= kTokenMaxRows ? cu_count(&cus) : H3A_OK;
+  if (rc) return rc;
+  if (!plan_token(a, cus)) {
+    a.nqt = (a.Sq + kRows - 1) / kRows;
+    const int grid = deal(a.nqt, a.B * a.H, &a.chunk);
+    hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
+    return check_launch("window_fwd_kernel");
+  }
+  a.part = static_cast<float *>(ws);
+  const int units = a.B * a.Hkv * a.nqt;
+  hipLaunchKernelGGL(window_token_kernel, dim3((unsigned)(units * a.pieces)), dim3(256), 0, s, a);
+  rc = check_launch("window_token_kernel");
+  if (rc || a.pieces == 1) return rc;
+  hipLaunchKernelGGL(window_token_sum_kernel, dim3((unsigned)(units * kTokenRows)), dim3(256), 0, s, a, units);
+  return check_launch("window_token_sum_kernel");
 }
 
 int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {

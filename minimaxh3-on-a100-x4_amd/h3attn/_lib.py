@@ -81,7 +81,9 @@ SIGNATURES = {
     "h3a_attn_fwd_blocksparse_tiles_ws": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                                                _c_i64_3, _c_i64_3, _c_i64_3, _c_i64_3, _vp, _vp, _i, _f,
                                                _vp, ctypes.c_size_t, _vp]),
-    "h3a_attn_fwd_window": (_i, [_vp] * 5 + [_i] * 6 + [_c_i64_3] * 4 + [ctypes.POINTER(Window), _f, _vp]),
+    "h3a_attn_fwd_window": (_i, [_vp] * 5 + [_i] * 6 + [_c_i64_3] * 4 + [ctypes.POINTER(Window), _f, _vp,
+                                                                         ctypes.c_size_t, _vp]),
+    "h3a_attn_fwd_window_workspace_size": (_i, [_i] * 6 + [ctypes.POINTER(Window), ctypes.POINTER(ctypes.c_size_t)]),
     "h3a_attn_bwd_window_workspace_size": (_i, [_i] * 6 + [ctypes.POINTER(Window), ctypes.POINTER(ctypes.c_size_t)]),
     "h3a_attn_bwd_window": (_i, [_vp] * 9 + [_i] * 6 + [_c_i64_3] * 8 + [ctypes.POINTER(Window), _f, _vp,
                                                                          ctypes.c_size_t, _vp]),

@@ -17,6 +17,10 @@ from ._lib import check, lib, strides3
 from .ops import HEAD_DIM, _as_kernel_input, _layout, _on_device, _stream
 
 
+# Query rows up to which the forward may split the keys, and need a workspace.
+SPLIT_ROWS = 256
+
+
 def _side(name: str, n) -> int:
     """A window side as an int; None is no limit."""
     if n is None:
@@ -105,9 +109,17 @@ def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, s
     lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device) if return_lse else None
     sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
     with _on_device(q):
+        ws, nbytes = None, 0
+        if Sq <= SPLIT_ROWS:
+            n = ctypes.c_size_t(0)
+            check("h3a_attn_fwd_window_workspace_size",
+                  lib().h3a_attn_fwd_window_workspace_size(B, H, Hkv, Sq, Skv, D, ctypes.byref(w), ctypes.byref(n)))
+            nbytes = n.value
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib().h3a_attn_fwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                        None if lse is None else lse.data_ptr(), B, H, Hkv, Sq, Skv, D, *st,
-                                       strides3(*ost), ctypes.byref(w), sc, _stream(q))
+                                       strides3(*ost), ctypes.byref(w), sc, None if ws is None else ws.data_ptr(), nbytes,
+                                       _stream(q))
     check("h3a_attn_fwd_window", rc)
     return (out, lse) if return_lse else out
 

@@ -16,7 +16,7 @@ ROW = S3(0, 0, 128)
 def _fwd(L, q=16, k=16, v=16, o=16, lse=None, B=1, H=2, Hkv=1, Sq=4, Skv=4, D=128, st=(ROW,) * 4,
          w=(3, 3, 1, 0, 0), starts=None, lens=None, scale=0.1):
     win = None if w is None else ctypes.byref(_lib.Window(*w, starts, lens))
-    return L.h3a_attn_fwd_window(q, k, v, o, lse, B, H, Hkv, Sq, Skv, D, *st, win, scale, None)
+    return L.h3a_attn_fwd_window(q, k, v, o, lse, B, H, Hkv, Sq, Skv, D, *st, win, scale, None, 0, None)
 
 
 def test_forward_refusals():
@@ -43,6 +43,18 @@ def test_forward_refusals():
         assert b"sequence stride" in L.h3a_last_error()
     assert _fwd(L, st=(ROW, ROW, ROW, S3(0, 0, 120))) == bad
     assert b"rows overlap" in L.h3a_last_error()
+
+
+def test_workspace_refusals():
+    L = _lib.lib()
+    n = ctypes.c_size_t(7)
+    w = ctypes.byref(_lib.Window(3, 3, 1, 0, 0, None, None))
+    size = L.h3a_attn_fwd_window_workspace_size
+    assert size(1, 2, 1, 40, 40, 128, w, None) == _lib.H3A_ERR_INVALID_ARG
+    assert size(1, 2, 1, 40, 40, 128, None, ctypes.byref(n)) == _lib.H3A_ERR_INVALID_ARG
+    assert size(1, 2, 1, 40, 40, 64, w, ctypes.byref(n)) == _lib.H3A_ERR_UNSUPPORTED
+    assert n.value == 7
+    assert size(1, 2, 1, 257, 300, 128, w, ctypes.byref(n)) == 0 and n.value == 0  # more than 256 rows: no split
 
 
 def test_backward_refusals():
