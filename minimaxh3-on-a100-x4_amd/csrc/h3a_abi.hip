@@ -288,7 +288,7 @@ int norm_affine(const char *name, const void *p, int w_dtype) {
 }
 
 size_t norm_bwd_bytes(const int *bounds, int segments, int C) {
-  const int wgs = norm_wgs(bounds, segments, norm_rows_per_wg(bounds[segments], C, kNormBwdWgs));
+  const int wgs = norm_wgs(bounds, segments, norm_rows_per_wg(bounds[segments], C, segments, true));
   return (size_t)wgs * 2 * C * sizeof(float);
 }
 
@@ -904,7 +904,7 @@ int h3a_layer_norm_fwd(const void *x, int64_t x_stride, const void *w, const voi
   a.w_add = modulate ? 1.f : 0.f;
   a.mean = mean; a.rstd = rstd;
   a.C = C; a.eps = eps;
-  a.rows_per_wg = norm_rows_per_wg(rows, C, kNormFwdWgs);
+  a.rows_per_wg = norm_rows_per_wg(rows, C, segments, false);
   return launch_layer_norm(a, bounds, segments, dtype, false, vec, as_stream(stream));
 }
 
@@ -948,7 +948,7 @@ int h3a_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t
   // Without rows no workgroup leaves a partial, and none is read; dw stands for "wanted".
   a.partial = need > 0 ? static_cast<float *>(workspace) : dw;
   a.C = C;
-  a.rows_per_wg = norm_rows_per_wg(rows, C, kNormBwdWgs);
+  a.rows_per_wg = norm_rows_per_wg(rows, C, segments, true);
   return launch_layer_norm(a, bounds, segments, dtype, true, vec, as_stream(stream));
 }
 

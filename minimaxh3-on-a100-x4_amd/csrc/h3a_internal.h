@@ -169,10 +169,7 @@ struct NormArgs {
   float eps;
   int bounds[kNormSegments + 1], first_wg[kNormSegments + 1];
 };
-// Workgroups the rows are shared among: forward, and backward, where each leaves a
-// partial row of the weights' gradients.
-constexpr int kNormFwdWgs = 2048, kNormBwdWgs = 512;
-int norm_rows_per_wg(int64_t rows, int C, int wgs);
+int norm_rows_per_wg(int64_t rows, int C, int segments, bool bwd);
 int norm_wgs(const int *bounds, int segments, int rows_per_wg);
 int launch_layer_norm(NormArgs a, const int *bounds, int segments, int dtype, bool bwd, bool vec, hipStream_t s);
 

@@ -52,15 +52,22 @@ __device__ __forceinline__ void unpack(const Row8<DT> &r, float (&x)[8]) {
 }
 
 // Channels c .. c+7 of a row of C; those past the end are 0.  VEC: C is a multiple of 8
-// and rows are 16-byte aligned.
+// and rows are 16-byte aligned; otherwise whole eights are read and written as 16-byte
+// accesses off their grid (which global memory takes) and a row's end one by one (60000
+// rows of 1001 bf16 channels, forward: 136 us with every channel by itself).
+template <int DT>
+__device__ __forceinline__ int64_t byte_of(int c) { return (int64_t)c * Row8<DT>::kBytes; }
 template <int DT, bool VEC>
 __device__ __forceinline__ Row8<DT> load8(const char *row, int c, int C) {
   Row8<DT> r;
+  constexpr int kVecs = sizeof(r.v) / sizeof(r.v[0]);
   if constexpr (VEC) {
-    constexpr int kVecs = sizeof(r.v) / sizeof(r.v[0]);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
-      r.v[i] = c < C ? *reinterpret_cast<const u32x4 *>(row + (int64_t)c * Row8<DT>::kBytes + 16 * i) : u32x4{0, 0, 0, 0};
+      r.v[i] = c < C ? *reinterpret_cast<const u32x4 *>(row + byte_of<DT>(c) + 16 * i) : u32x4{0, 0, 0, 0};
+  } else if (c + 8 <= C) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) __builtin_memcpy(&r.v[i], row + byte_of<DT>(c) + 16 * i, 16);
   } else if constexpr (DT == H3A_FP32) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -91,13 +98,15 @@ __device__ __forceinline__ void store8(char *row, int c, int C, const float (&x)
       r.v[0][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
     }
   }
+  constexpr int kVecs = sizeof(r.v) / sizeof(r.v[0]);
   if constexpr (VEC) {
-    constexpr int kVecs = sizeof(r.v) / sizeof(r.v[0]);
     if (c < C) {
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-        *reinterpret_cast<u32x4 *>(row + (int64_t)c * Row8<DT>::kBytes + 16 * i) = r.v[i];
+      for (int i = 0; i < kVecs; ++i) *reinterpret_cast<u32x4 *>(row + byte_of<DT>(c) + 16 * i) = r.v[i];
     }
+  } else if (c + 8 <= C) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) __builtin_memcpy(row + byte_of<DT>(c) + 16 * i, &r.v[i], 16);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -226,25 +235,49 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(NormArgs a) {
     for (int e = 0; e < 8; ++e) dw[i][e] = db[i][e] = 0.f;
   }
   const float inv_c = 1.f / (float)a.C;
-  int slot = 0;
-  for (int r = sh.r0 + (int)threadIdx.x / TPR; r < sh.r1; r += kRowsAtOnce) {
+  // The next row's loads are in flight while a row is reduced and stored, where
+  // registers allow; a row itself stays as it came from memory and is unpacked twice, so
+  // the loads fit (42120 rows of 5376 bf16 channels: 427 us without the loads ahead, 388
+  // with them and floats kept, 335 so).
+  constexpr bool kAhead = NV * sizeof(Row8<DT>) <= 48;
+  Row8<DT> xn[NV], gn[NV];
+  float mean_n = 0.f, rstd_n = 0.f;
+  auto load = [&](int r) __attribute__((always_inline)) {
     const char *xr = a.x + (int64_t)r * a.x_stride, *gr = a.dy + (int64_t)r * a.dy_stride;
-    const float mean = a.mean[r], rstd = a.rstd[r];
-    float xh[NV][8], g[NV][8];
+    mean_n = a.mean[r];
+    rstd_n = a.rstd[r];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      xn[i] = load8<DT, VEC>(xr, 8 * (t + i * TPR), a.C);
+      gn[i] = load8<DT, VEC>(gr, 8 * (t + i * TPR), a.C);
+    }
+  };
+  int slot = 0, r = sh.r0 + (int)threadIdx.x / TPR;
+  if (kAhead && r < sh.r1) load(r);
+  for (; r < sh.r1; r += kRowsAtOnce) {
+    if (!kAhead) load(r);
+    const float mean = mean_n, rstd = rstd_n;
+    Row8<DT> xc[NV], gc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      xc[i] = xn[i];
+      gc[i] = gn[i];
+    }
+    if (kAhead && r + kRowsAtOnce < sh.r1) load(r + kRowsAtOnce);
     float2 s = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (t + i * TPR);
-      unpack<DT>(load8<DT, VEC>(xr, c, a.C), xh[i]);
-      unpack<DT>(load8<DT, VEC>(gr, c, a.C), g[i]);
+      float x[8], g[8];
+      unpack<DT>(xc[i], x);
+      unpack<DT>(gc[i], g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        xh[i][e] = (xh[i][e] - mean) * rstd;
-        dw[i][e] = fmaf(g[i][e], xh[i][e], dw[i][e]);
-        db[i][e] += g[i][e];
-        g[i][e] *= w[i][e];
-        s.x += g[i][e];
-        s.y = fmaf(g[i][e], xh[i][e], s.y);
+        x[e] = (x[e] - mean) * rstd;
+        dw[i][e] = fmaf(g[e], x[e], dw[i][e]);
+        db[i][e] += g[e];
+        g[e] *= w[i][e];
+        s.x += g[e];
+        s.y = fmaf(g[e], x[e], s.y);
       }
     }
     s = row_sum<TPR>(s, xch, slot);
@@ -253,10 +286,16 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(NormArgs a) {
     char *dr = a.y + (int64_t)r * a.y_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = rstd * (g[i][e] - m1 - xh[i][e] * m2);
-      store8<DT, VEC>(dr, 8 * (t + i * TPR), a.C, d);
+      for (u32x4 &v : xc[i].v) asm volatile("" : "+v"(v));  // unpacked again, not kept
+#pragma unroll
+      for (u32x4 &v : gc[i].v) asm volatile("" : "+v"(v));
+      float x[8], g[8];
+      unpack<DT>(xc[i], x);
+      unpack<DT>(gc[i], g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = rstd * (g[e] * w[i][e] - m1 - (x[e] - mean) * rstd * m2);
+      store8<DT, VEC>(dr, 8 * (t + i * TPR), a.C, x);
     }
   }
   if (!a.partial) return;
@@ -295,8 +334,17 @@ __global__ void __launch_bounds__(256) layer_norm_param_grad_kernel(NormArgs a) 
   const int c = blockIdx.x * 64 + lane, seg = blockIdx.y, which = blockIdx.z;
   const int w0 = a.wg0 + a.first_wg[seg], w1 = a.wg0 + a.first_wg[seg + 1];
   float sum = 0.f;
-  if (c < a.C)
-    for (int w = w0 + wave; w < w1; w += 4) sum += a.partial[((int64_t)w * 2 + which) * a.C + c];
+  if (c < a.C) {
+    constexpr int kFlight = 8;  // loads in flight
+    for (int w = w0 + wave; w < w1; w += 4 * kFlight) {
+      float v[kFlight];
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i)
+        v[i] = w + 4 * i < w1 ? a.partial[((int64_t)(w + 4 * i) * 2 + which) * a.C + c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) sum += v[i];
+    }
+  }
   fold[wave][lane] = sum;
   __syncthreads();
   if (wave == 0 && c < a.C)
@@ -339,9 +387,12 @@ NormKernel pick(int dtype, int C, int *rows_at_once) {
 
 }  // namespace
 
-// Rows per workgroup: so many that `wgs` workgroups share all the rows (each segment
-// adds at most one more), in whole steps of the rows it takes at once.
-int norm_rows_per_wg(int64_t rows, int C, int wgs) {
+// Rows per workgroup, in whole steps of the rows it takes at once: as many as make the
+// workgroups just fit the chip's 256 CUs at once, each segment adding at most one (13
+// more than fit took 408 us for 335 at 42120 rows of 5376 channels, backward).
+int norm_rows_per_wg(int64_t rows, int C, int segments, bool bwd) {
+  const int per_cu = bwd ? (C <= 512 || (C > 1024 && C <= 2048) ? 5 : (C <= 1024 ? 3 : 2)) : (C <= 2048 ? 8 : 4);
+  const int wgs = 256 * per_cu - (segments < 128 ? segments : 0);
   const int step = C <= 1024 ? 4 : 1;
   const int64_t n = (rows + wgs - 1) / wgs;
   return (int)((n < 1 ? 1 : n) + step - 1) / step * step;

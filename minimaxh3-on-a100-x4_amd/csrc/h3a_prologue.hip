@@ -491,26 +491,33 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(RopeAxesArgs a) {
   }
 }
 
-// Sums of the workgroups' partial rows in a fixed order: 16 columns per workgroup, 16
-// lanes to a column, each taking every sixteenth row.
+// Sums of the workgroups' partial rows in a fixed order: 4 columns per workgroup, 64
+// threads to a column, each taking every 64th row, all in flight.
+constexpr int kAxesBwdWgs = 768;  // 3 workgroups of the backward kernel per CU at a time
 __global__ void __launch_bounds__(256) rope_axes_param_grad_kernel(RopeAxesArgs a, int wgs) {
-  __shared__ float fold[16][17];
-  const int col = threadIdx.x & 15, part = threadIdx.x >> 4, at = blockIdx.x * 16 + col;
-  float sum = 0.f;
-  for (int i = part; i < wgs; i += 16) sum += a.partial[(int64_t)i * 256 + at];
-  fold[part][col] = sum;
-  __syncthreads();
-  if (part == 0) {
-    sum = 0.f;
-    for (int i = 0; i < 16; ++i) sum += fold[i][col];
-    a.dw[at >> 7][at & 127] = sum;
+  __shared__ float fold[4][4];
+  const int col = threadIdx.x & 3, part = threadIdx.x >> 2, at = blockIdx.x * 4 + col;
+  constexpr int kPer = kAxesBwdWgs / 64;
+  float v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int row = part + 64 * i;
+    v[i] = row < wgs ? a.partial[(int64_t)row * 256 + at] : 0.f;
   }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += v[i];
+#pragma unroll
+  for (int o = 4; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  if ((threadIdx.x & 63) < 4) fold[threadIdx.x >> 6][col] = sum;
+  __syncthreads();
+  if (threadIdx.x < 4) a.dw[at >> 7][at & 127] = (fold[0][col] + fold[1][col]) + (fold[2][col] + fold[3][col]);
 }
 
 // Backward: workgroups that each leave a partial row of the weights' gradients.
 int rope_axes_bwd_wgs(int B, int S) {
   const int64_t n = ((int64_t)B * S + kAxesTokens - 1) / kAxesTokens;
-  return (int)(n < 1024 ? n : 1024);
+  return (int)(n < kAxesBwdWgs ? n : kAxesBwdWgs);
 }
 
 template <bool kBwd>
@@ -525,7 +532,7 @@ static int launch_rope_axes_as(const RopeAxesArgs &a, hipStream_t s) {
   hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(256), 0, s, a);
   int rc = check_launch("rope_axes_kernel");
   if (rc || !kBwd) return rc;
-  hipLaunchKernelGGL(rope_axes_param_grad_kernel, dim3(16), dim3(256), 0, s, a, (int)wgs);
+  hipLaunchKernelGGL(rope_axes_param_grad_kernel, dim3(64), dim3(256), 0, s, a, (int)wgs);
   return check_launch("rope_axes_param_grad_kernel");
 }
 int launch_rope_axes(const RopeAxesArgs &a, bool bwd, hipStream_t s) {
