@@ -42,23 +42,117 @@ struct DualLayout {
     const int c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     return (4 * g + i) * kVRow + 16 * (c ^ (4 * i + g)) + 8 * (lane & 1);
   }
+  __device__ __forceinline__ static int v_off(int vb, int dt) { return vb ^ (64 * dt); }
+  __device__ __forceinline__ static int v_off8(int off) { return off ^ 32; }  // 8 rows on, less 8 * kVRow
+};
+struct ValueLayout : SwzLayout {
+  __device__ __forceinline__ static int v_off8(int off) { return off; }
 };
 
-// acc (128 dims x 32 columns) += X^T P over NKS sixteen-row steps of tile X, P in the
-// score accumulator's order (pack_p).
-template <int NKS>
-__device__ __forceinline__ void transposed_product(const uint16_t *buf, const u32x4 (&pf)[NKS], int v_rd,
-                                                   f32x16 (&acc)[4]) {
-  const char *vb = reinterpret_cast<const char *>(buf);
+// MFMAs fed from LDS in a fixed order: an operand is read kAhead instructions before the
+// MFMA that takes it (left to itself the compiler reads one or two ahead and every MFMA
+// waits for LDS: 40-55 % of the matrix cores' cycles).  pin_order() keeps what is written
+// before it before what is written after it.
+__device__ __forceinline__ void pin_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Operand i of the scores of a 64-row stage X: rows 32 * (i % 2) .., k-step i / 2.
+template <class L>
+__device__ __forceinline__ u32x4 stage_operand(const uint16_t *x, int k_rd, int i) {
+  return *(const u32x4 *)(reinterpret_cast<const char *>(x) + L::k_off(k_rd, i >> 1) + (i & 1) * 32 * 256);
+}
+// The transposed operand of acc[i % 4] for 16-row step i / 4 of tile X.
+template <class L>
+__device__ __forceinline__ u32x4 transposed_operand(const uint16_t *x, int t_rd, int i) {
+  const char *p = reinterpret_cast<const char *>(x) + 16 * (i >> 2) * 256;
+  const int off = L::v_off(t_rd, i & 3);
+  const u32x2 lo = lds_read_tr16_b64(reinterpret_cast<const uint16_t *>(p + off));
+  const u32x2 hi = lds_read_tr16_b64(reinterpret_cast<const uint16_t *>(p + L::v_off8(off) + 8 * 256));
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+constexpr int kAhead = 6, kAheadT = 3;
+
+// acc += X^T F for a wave's 32 columns, where F = weigh(s) of the scores s = X xf over the
+// 64 rows of a stage; the product is with Y.
+template <class LX, class LY, class Weigh>
+__device__ __forceinline__ void stage_single(const uint16_t *x, const uint16_t *y, const u32x4 (&xf)[8], int k_rd,
+                                             int t_rd, f32x16 (&acc)[4], Weigh weigh) {
+  f32x16 s[2] = {f32x16{0.f}, f32x16{0.f}};
+  u32x4 a[kAhead], b[kAheadT], f[4];
+  pin_order();
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
+  for (int i = 0; i < kAhead; ++i) a[i] = stage_operand<LX>(x, k_rd, i);
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
-      const int off = v_rd ^ (64 * dt);
-      const u32x2 lo = lds_read_tr16_b64(reinterpret_cast<const uint16_t *>(vb + off + 16 * ks * 256));
-      const u32x2 hi = lds_read_tr16_b64(reinterpret_cast<const uint16_t *>(vb + (off ^ 32) + (16 * ks + 8) * 256));
-      acc[dt] = mfma_32x32x16(u32x4{lo.x, lo.y, hi.x, hi.y}, pf[ks], acc[dt]);
+  for (int i = 0; i < 16; ++i) {
+    pin_order();
+    s[i & 1] = mfma_32x32x16(a[i % kAhead], xf[i >> 1], s[i & 1]);
+    if (i + kAhead < 16) a[i % kAhead] = stage_operand<LX>(x, k_rd, i + kAhead);
+  }
+#pragma unroll
+  for (int i = 0; i < kAheadT; ++i) b[i] = transposed_operand<LY>(y, t_rd, i);
+  pin_order();
+  weigh(s, f);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    pin_order();
+    acc[i & 3] = mfma_32x32x16(b[i % kAheadT], f[i >> 2], acc[i & 3]);
+    if (i + kAheadT < 16) b[i % kAheadT] = transposed_operand<LY>(y, t_rd, i + kAheadT);
+  }
+  pin_order();
+}
+
+// The same with F = weigh(s, dp) of two scores, s = X xf and dp = Y yf, and the product
+// with X: 32 rows at a time, the two chains of MFMAs side by side.
+template <class L, class Weigh>
+__device__ __forceinline__ void stage_pair(const uint16_t *x, const uint16_t *y, const u32x4 (&xf)[8],
+                                           const u32x4 (&yf)[8], int k_rd, int t_rd, f32x16 (&acc)[4], Weigh weigh) {
+  auto operand = [&](int u, int i) __attribute__((always_inline)) {
+    return *(const u32x4 *)(reinterpret_cast<const char *>(i & 1 ? y : x) + L::k_off(k_rd, i >> 1) + u * 32 * 256);
+  };
+  u32x4 a[kAhead];
+  pin_order();
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) a[i] = operand(0, i);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    f32x16 s = {0.f}, dp = {0.f};
+    u32x4 b[kAheadT], f[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      pin_order();
+      if (i & 1) dp = mfma_32x32x16(a[i % kAhead], yf[i >> 1], dp);
+      else s = mfma_32x32x16(a[i % kAhead], xf[i >> 1], s);
+      if (i + kAhead < 16) a[i % kAhead] = operand(u, i + kAhead);
     }
+#pragma unroll
+    for (int i = 0; i < kAheadT; ++i) b[i] = transposed_operand<L>(x + u * 32 * 128, t_rd, i);
+    pin_order();
+    weigh(u, s, dp, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      pin_order();
+      acc[i & 3] = mfma_32x32x16(b[i % kAheadT], f[i >> 2], acc[i & 3]);
+      if (i + kAheadT < 8) {
+        b[i % kAheadT] = transposed_operand<L>(x + u * 32 * 128, t_rd, i + kAheadT);
+      } else if (u == 0) {  // the other half's first operands
+        a[2 * (i + kAheadT - 8)] = operand(1, 2 * (i + kAheadT - 8));
+        a[2 * (i + kAheadT - 8) + 1] = operand(1, 2 * (i + kAheadT - 8) + 1);
+      }
+    }
+  }
+  pin_order();
+}
+static_assert(kAhead == 2 * kAheadT, "stage_pair: the last products fetch the next scores' operands");
+
+// Stages 0 .. n-1 of two LDS buffers in turn, as code of their own, so that every LDS
+// address is a register and a constant.
+template <int P>
+using C = std::integral_constant<int, P>;
+template <class Stage>
+__device__ __forceinline__ void two_buffers(int n, Stage stage) {
+  for (int j = 0; j < n; j += 2) {
+    stage(C<0>{}, j);
+    if (j + 1 < n) stage(C<1>{}, j + 1);
   }
 }
 
@@ -230,30 +324,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     TileDma<4, L, true> vdma;
     kdma.init(a.kss, wave, lane);
     vdma.init(a.vss, wave, lane);
-    auto fetch = [&](int j) __attribute__((always_inline)) {
-      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), kbuf[j & 1]);
-      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), vbuf[j & 1]);
+    auto fetch = [&](int j, auto par) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), kbuf[P]);
+      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
     };
-    fetch(0);
+    fetch(0, C<0>{});
     u32x4 qf[8];
     load_columns(qf, a.q + it.b * a.qsb + it.h * a.qsh, a.qss, row, a.Sq, g);
     const int k_rd = L::k_base(l32, g), v_rd = L::v_base(lane);
     wait_vmem_all();
     __syncthreads();
-    for (int j = 0; j < st.n; ++j) {
-      if (j + 1 < st.n) fetch(j + 1);
+    two_buffers(st.n, [&](auto par, int j) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      if (j + 1 < st.n) fetch(j + 1, C<P ^ 1>{});
       const Cover c = cover_of(a, sp, st, j, p0, p1);
-      if (c != kNone) {
-        f32x16 s[2];
-        u32x4 pf[4];
-        score_tile<L, 2>(kbuf[j & 1], qf, k_rd, s);
-        if (c == kPart) mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, kNegInf);
-        softmax_stage<2>(s, 0, kBN, g, a.sl2, m, lsum, o, pf);
-        pv_tile<L, 4>(vbuf[j & 1], pf, v_rd, o);
-      }
+      if (c != kNone)
+        stage_single<L, ValueLayout>(kbuf[P], vbuf[P], qf, k_rd, v_rd, o,
+                                     [&](f32x16(&s)[2], u32x4(&pf)[4]) __attribute__((always_inline)) {
+                                       if (c == kPart) mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, kNegInf);
+                                       softmax_stage<2>(s, 0, kBN, g, a.sl2, m, lsum, o, pf);
+                                     });
       wait_vmem_all();
       __syncthreads();
-    }
+    });
   }
   const float ltot = half_swap_sum(lsum);
   const float inv = ltot > 0.f ? 1.f / ltot : 0.f;
@@ -474,11 +568,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     TileDma<4, L, false> kdma, vdma;
     kdma.init(a.kss, wave, lane);
     vdma.init(a.vss, wave, lane);
-    auto fetch = [&](int j) __attribute__((always_inline)) {
-      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), kbuf[j & 1]);
-      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), vbuf[j & 1]);
+    auto fetch = [&](int j, auto par) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), kbuf[P]);
+      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
     };
-    fetch(0);
+    fetch(0, C<0>{});
     u32x4 qf[8], df[8];
     load_columns(qf, a.q + it.b * a.qsb + it.h * a.qsh, a.qss, row, a.Sq, g);
     load_columns(df, a.dout + it.b * a.gsb + it.h * a.gsh, a.gss, row, a.Sq, g);
@@ -502,27 +597,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
     wait_vmem_all();
     __syncthreads();
-    for (int j = 0; j < st.n; ++j) {
-      if (j + 1 < st.n) fetch(j + 1);
+    two_buffers(st.n, [&](auto par, int j) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      if (j + 1 < st.n) fetch(j + 1, C<P ^ 1>{});
       const Cover c = cover_of(a, sp, st, j, p0, p1);
-      if (c != kNone) {
-        f32x16 s[2], dp[2];
-        u32x4 dsf[4];
-        score_tile<L, 2>(kbuf[j & 1], qf, k_rd, s);
-        if (c == kPart) mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, kNegInf);
-        score_tile<L, 2>(vbuf[j & 1], df, k_rd, dp);
+      if (c != kNone)
+        stage_pair<L>(kbuf[P], vbuf[P], qf, df, k_rd, t_rd, dq,
+                      [&](int u, f32x16 &s, const f32x16 &dp, u32x4 (&f)[2]) __attribute__((always_inline)) {
+                        f32x16 ds[1];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+                        for (int r = 0; r < 16; ++r)
+                          ds[0][r] = fast_exp2(fmaf(s[r], a.sl2, -l2)) * (dp[r] - delta);
+                        if (c == kPart) {
+                          const int key0 = st.key0(j) + 32 * u + 4 * g, low = j < st.n_first ? 1 << 30 : lo;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[u][r] = fast_exp2(fmaf(s[u][r], a.sl2, -l2)) * (dp[u][r] - delta);
-        // (0 * dP is not 0 where a hidden value row holds an infinity or NaN.)
-        if (c == kPart) mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, 0.f);
-        pack_p<2>(s, dsf);
-        transposed_product<4>(kbuf[j & 1], dsf, t_rd, dq);
-      }
+                          for (int r = 0; r < 16; ++r) {
+                            const int at = key0 + 8 * (r >> 2) + (r & 3);
+                            if (!((at >= low && at <= hi) || at < first)) ds[0][r] = 0.f;
+                          }
+                        }
+                        pack_p<1>(ds, f);
+                      });
       wait_vmem_all();
       __syncthreads();
-    }
+    });
   }
   if (wq0 < a.Sq)
     store_columns(dq, a.scale, live, reinterpret_cast<uint8_t *>(&kbuf[0][0]) + wave * 8192,
@@ -543,8 +641,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 //
 // The first keys are seen by every query, the others by a window's: tiles that hold
 // first keys are cut into a.pieces equal runs of stages, which leave fp32 partial sums
-// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being the shortest,
-// and dK before dV.
+// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being the shortest.
 constexpr int kQStage = 64;
 struct DkdvLds {
   uint16_t q[2][kQStage * 128], dout[2][kQStage * 128];
@@ -590,7 +687,8 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
     ddma.init(a.gss, wave, lane);
     int fh = it.h * a.rep + (int)(t_a / per_head), frow = i_a + (int)(t_a % per_head) * kQStage;
     int crow = frow;  // rows of the stage that is computed
-    auto fetch = [&](int slot) __attribute__((always_inline)) {
+    auto fetch = [&](auto par) __attribute__((always_inline)) {
+      constexpr int slot = decltype(par)::value;
       qdma.issue(a.q + it.b * a.qsb + fh * a.qsh, a.qss, frow, i_b, lds.q[slot]);
       ddma.issue(a.dout + it.b * a.gsb + fh * a.gsh, a.gss, frow, i_b, lds.dout[slot]);
       // Rows past i_b are zeros throughout: p = 1, but dO = dP = delta = 0.
@@ -605,8 +703,8 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
         ++fh;
       }
     };
-    fetch(0);
-    u32x4 kf[8], vf[kDk ? 8 : 1];
+    fetch(C<0>{});
+    u32x4 kf[8], vf[8];
     load_columns(kf, a.k + it.b * a.ksb + it.h * a.ksh, a.kss, key, sp.len, g);
     if constexpr (kDk) load_columns(vf, a.v + it.b * a.vsb + it.h * a.vsh, a.vss, key, sp.len, g);
     const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
@@ -624,59 +722,60 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
       }
       return keys_whole && p0 >= wj0 + 31 - a.right && p1 <= (wj0 < a.sinks ? a.sinks : wj0) + a.left ? kAll : kPart;
     };
-    // Row statistics of accumulator registers 4*r4 .. 4*r4+3 of sub-tile u.
+    // Statistic `which` of the rows of accumulator registers 4*r4 .. 4*r4+3 of half u.
     auto row_stats = [&](int slot, int which, int u, int r4, float(&x)[4]) __attribute__((always_inline)) {
       const float4 v = *(const float4 *)&lds.stats[slot][which][32 * u + 8 * r4 + 4 * g];
       x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     };
     wait_vmem_all();
     __syncthreads();
-    for (int j = 0; j < n; ++j) {
-      const int slot = j & 1, p0 = sp.qs + crow;
+    two_buffers(n, [&](auto par, int j) __attribute__((always_inline)) {
+      constexpr int slot = decltype(par)::value;
+      const int p0 = sp.qs + crow;
       crow += kQStage;
       if (crow >= i_b) crow = i_a;
-      if (j + 1 < n) fetch(slot ^ 1);
+      if (j + 1 < n) fetch(C<slot ^ 1>{});
       const Cover c = cover(p0);
-      if (c != kNone) {
-        f32x16 s[2];
-        u32x4 f[4];
-        score_tile<L, 2>(lds.q[slot], kf, k_rd, s);
+      // Half u's scores -> p, or (dK) ds; 0 where the row does not see the key.
+      auto weigh = [&](int u, f32x16 &s, const f32x16 *dp) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int r4 = 0; r4 < 4; ++r4) {
+          float l2[4], de[4];
+          row_stats(slot, 0, u, r4, l2);
+          if (kDk) row_stats(slot, 1, u, r4, de);
 #pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            float l2[4];
-            row_stats(slot, 0, u, r4, l2);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[u][4 * r4 + r] = fast_exp2(fmaf(s[u][4 * r4 + r], a.sl2, -l2[r]));
+          for (int r = 0; r < 4; ++r) {
+            const float p = fast_exp2(fmaf(s[4 * r4 + r], a.sl2, -l2[r]));
+            s[4 * r4 + r] = kDk ? p * ((*dp)[4 * r4 + r] - de[r]) : p;
           }
+        }
+        if (c == kPart) {
+          const uint32_t ahead = (uint32_t)(p0 + 32 * u + 4 * g - plo);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (ahead + 8 * (r >> 2) + (r & 3) > span) s[r] = 0.f;
+        }
+      };
+      if (c != kNone) {
         if constexpr (kDk) {
-          f32x16 dp[2];
-          score_tile<L, 2>(lds.dout[slot], vf, k_rd, dp);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-              float de[4];
-              row_stats(slot, 1, u, r4, de);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) s[u][4 * r4 + r] *= dp[u][4 * r4 + r] - de[r];
-            }
+          stage_pair<L>(lds.q[slot], lds.dout[slot], kf, vf, k_rd, t_rd, acc,
+                        [&](int u, f32x16 &s, const f32x16 &dp, u32x4(&f)[2]) __attribute__((always_inline)) {
+                          weigh(u, s, &dp);
+                          const f32x16 ds[1] = {s};
+                          pack_p<1>(ds, f);
+                        });
+        } else {
+          stage_single<L, L>(lds.q[slot], lds.dout[slot], kf, k_rd, t_rd, acc,
+                             [&](f32x16(&s)[2], u32x4(&f)[4]) __attribute__((always_inline)) {
+                               weigh(0, s[0], nullptr);
+                               weigh(1, s[1], nullptr);
+                               pack_p<2>(s, f);
+                             });
         }
-        if (c == kPart) {  // p or ds of rows that do not see the key
-          const uint32_t ahead = (uint32_t)(p0 + 4 * g - plo);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (ahead + 32 * u + 8 * (r >> 2) + (r & 3) > span) s[u][r] = 0.f;
-        }
-        pack_p<2>(s, f);
-        transposed_product<4>(kDk ? lds.q[slot] : lds.dout[slot], f, t_rd, acc);
       }
       wait_vmem_all();
       __syncthreads();
-    }
+    });
   }
   if (piece >= 0) {
     const int64_t bh = (int64_t)it.b * a.Hkv + it.h;
@@ -698,15 +797,16 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
 
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dkdv_kernel(WindowArgs a) {
   __shared__ __attribute__((aligned(16))) DkdvLds lds;
-  // The grid: dK and dV of the whole tiles, then dK and dV of the pieces.
+  // The grid: the whole tiles, then the pieces; each run of tiles once for dK and then
+  // for dV, which read the same rows.
   int i = (int)blockIdx.x;
   const bool whole = i < 2 * a.grid_whole;
   if (!whole) i -= 2 * a.grid_whole;
-  const int half = whole ? a.grid_whole : a.grid_pieces;
-  const bool dv = i >= half;
-  if (dv) i -= half;
-  Item it = whole ? item_of(a, i, a.chunk, a.nkt - a.first_tiles, a.Hkv)
-                  : item_of(a, i, a.chunk_pieces, a.first_tiles * a.pieces, a.Hkv);
+  const int chunk = whole ? a.chunk : a.chunk_pieces, k = i >> 3;
+  const bool dv = (k / chunk) & 1;
+  i = ((k / (2 * chunk) * chunk + k % chunk) << 3) | (i & 7);  // without the dK, dV pairing
+  Item it = whole ? item_of(a, i, chunk, a.nkt - a.first_tiles, a.Hkv)
+                  : item_of(a, i, chunk, a.first_tiles * a.pieces, a.Hkv);
   if (it.tile < 0) return;
   int piece = -1;  // of tile it.tile
   if (whole) {
@@ -765,10 +865,10 @@ size_t window_bwd_bytes(WindowArgs a) {
   return 2 * stat_rows(a) * sizeof(float) + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
 }
 
-// Grid of `tiles` work items for each of `heads` heads (item_of).
-static int deal(int tiles, int heads, int *chunk) {
-  const int64_t total = (int64_t)heads * tiles;
-  *chunk = total / 512 < 1 ? 1 : (total / 512 > 16 ? 16 : (int)(total / 512));
+// Grid of `tiles` work items for each of `heads` heads (item_of), in `runs` runs or more.
+static int deal(int tiles, int heads, int runs_wanted, int *chunk) {
+  const int64_t total = (int64_t)heads * tiles, most = total / runs_wanted;
+  *chunk = most < 1 ? 1 : (most > 16 ? 16 : (int)most);
   const int64_t runs = (int64_t)heads * ((tiles + *chunk - 1) / *chunk);
   return (int)((runs + 7) / 8 * 8 * *chunk);
 }
@@ -825,7 +925,7 @@ int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
   if (rc) return rc;
   if (!plan_token(a, cus)) {
     a.nqt = (a.Sq + kRows - 1) / kRows;
-    const int grid = deal(a.nqt, a.B * a.H, &a.chunk);
+    const int grid = deal(a.nqt, a.B * a.H, 512, &a.chunk);
     hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
     return check_launch("window_fwd_kernel");
   }
@@ -838,18 +938,19 @@ int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
   return check_launch("window_token_sum_kernel");
 }
 
+constexpr int kKeyRuns = 128;
 int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {
   a.stats = static_cast<float *>(ws);
   a.stats_n = (int64_t)stat_rows(a);
   a.nqt = (a.Sq + kRows - 1) / kRows;
-  const int grid = deal(a.nqt, a.B * a.H, &a.chunk);
+  const int grid = deal(a.nqt, a.B * a.H, 512, &a.chunk);
   hipLaunchKernelGGL(window_dq_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   int rc = check_launch("window_dq_kernel");
   if (rc) return rc;
   plan_dkdv(a);
   a.part = a.stats + 2 * a.stats_n;
-  a.grid_whole = deal(a.nkt - a.first_tiles, a.B * a.Hkv, &a.chunk);
-  a.grid_pieces = deal(a.first_tiles * a.pieces, a.B * a.Hkv, &a.chunk_pieces);
+  a.grid_whole = deal(a.nkt - a.first_tiles, a.B * a.Hkv, kKeyRuns, &a.chunk);
+  a.grid_pieces = deal(a.first_tiles * a.pieces, a.B * a.Hkv, kKeyRuns, &a.chunk_pieces);
   hipLaunchKernelGGL(window_dkdv_kernel, dim3((unsigned)(2 * a.grid_whole + 2 * a.grid_pieces)), dim3(256), 0, s, a);
   rc = check_launch("window_dkdv_kernel");
   if (rc || a.first_tiles == 0) return rc;
