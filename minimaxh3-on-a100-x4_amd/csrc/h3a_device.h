@@ -142,6 +142,15 @@ __device__ __forceinline__ u32x4 range_desc(const void *p, int bytes) {
                (uint32_t)__builtin_amdgcn_readfirstlane(bytes), (uint32_t)kBufferConfig};
 }
 
+// A descriptor ready for the inline-asm loads above.  A vector instruction's scalar
+// result (readfirstlane) may be read by a vector-memory instruction five wait states
+// later at the earliest; the compiler keeps that distance to its own loads only, and a
+// load that comes too early sees the register's old value, an empty range for one.
+__device__ __forceinline__ u32x4 settled(u32x4 desc) {
+  asm volatile("s_nop 4" : "+s"(desc));
+  return desc;
+}
+
 // s_waitcnt vmcnt(N): at most the N most recent vector-memory loads of this
 // wave (LDS DMA included) are still in flight; loads complete in order.  The
 // other counters are left alone (expcnt 7, lgkmcnt 15).

@@ -195,6 +195,13 @@ __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul,
   }
 }
 
+// DMA of the rows of [row0, limit) that a tile holds, the rest as zeros.
+template <class Dma>
+__device__ __forceinline__ void fetch_tile(const Dma &dma, const uint16_t *base, int64_t stride, int row0, int limit,
+                                           uint16_t *tile) {
+  dma.template issue_desc<0, Dma::kInst>(settled(dma.desc(base, stride, row0, limit)), tile);
+}
+
 // A sequence of the batch: first query's position, keys, and the rows that are tokens.
 struct Span {
   int qs, len, i_lo, i_hi;  // rows i_lo <= i < i_hi sit at positions 0 <= qs + i < len
@@ -326,8 +333,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     vdma.init(a.vss, wave, lane);
     auto fetch = [&](int j, auto par) __attribute__((always_inline)) {
       constexpr int P = decltype(par)::value;
-      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), kbuf[P]);
-      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
+      fetch_tile(kdma, Kb, a.kss, st.key0(j), st.limit(j), kbuf[P]);
+      fetch_tile(vdma, Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
     };
     fetch(0, C<0>{});
     u32x4 qf[8];
@@ -369,9 +376,20 @@ struct TokenLds {
   uint16_t k[4][2][kTokenStage * 128], v[4][2][kTokenStage * 128];  // by wave
 };
 
-// Column of a workgroup's rows -> query row and head.
-__device__ __forceinline__ int token_row(const WindowArgs &a, int col) { return col % a.Sq; }
-__device__ __forceinline__ int token_head(const WindowArgs &a, int col) { return col / a.Sq; }
+// Column c of a key head's group of 32 -> query row and head among those that share it
+// (row >= Sq: none).  Sequences of 32 rows or more fill groups head by head, so that a
+// group's rows are consecutive; shorter ones run on from head to head.
+struct TokenColumn {
+  int row, head;
+};
+__device__ __forceinline__ TokenColumn token_column(const WindowArgs &a, int group, int c) {
+  if (a.Sq >= kTokenRows) {
+    const int per_head = (a.Sq + kTokenRows - 1) / kTokenRows;
+    return {group % per_head * kTokenRows + c, group / per_head};
+  }
+  const int col = group * kTokenRows + c;
+  return {col < a.rep * a.Sq ? col % a.Sq : a.Sq, col / a.Sq};
+}
 
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) window_token_kernel(WindowArgs a) {
   using L = SwzLayout;
@@ -381,10 +399,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
   const int piece = (int)blockIdx.x % a.pieces, unit = (int)blockIdx.x / a.pieces;
   const int group = unit % a.nqt, bh = unit / a.nqt, hk = bh % a.Hkv, b = bh / a.Hkv;
   const Span sp = span_of(a, b);
-  const int col = group * kTokenRows + l32;
-  const bool has = col < a.rep * a.Sq;
-  const int h = hk * a.rep + (has ? token_head(a, col) : 0), row = has ? token_row(a, col) : 0;
-  const int r0 = sp.i_lo, r1 = sp.i_hi - 1;
+  const TokenColumn at = token_column(a, group, l32);
+  const bool has = at.row < a.Sq;
+  const int h = hk * a.rep + (has ? at.head : 0), row = has ? at.row : 0;
+  // The rows the workgroup's keys are for: its 32, or all of a short sequence.
+  const int c0 = a.Sq < kTokenRows ? 0 : __builtin_amdgcn_readfirstlane(token_column(a, group, 0).row);
+  const int r0 = c0 > sp.i_lo ? c0 : sp.i_lo, r1 = (c0 + kTokenRows < sp.i_hi ? c0 + kTokenRows : sp.i_hi) - 1;
   const bool live = has && row >= r0 && row <= r1;
 
   f32x16 o[4];
@@ -406,8 +426,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
     vdma.init(a.vss, 0, lane);
     constexpr int kInst = decltype(kdma)::kInst + decltype(vdma)::kInst;
     auto fetch = [&](int j, int buf) __attribute__((always_inline)) {
-      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), lds.k[wave][buf]);
-      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), lds.v[wave][buf]);
+      fetch_tile(kdma, Kb, a.kss, st.key0(j), st.limit(j), lds.k[wave][buf]);
+      fetch_tile(vdma, Vb, a.vss, st.key0(j), st.limit(j), lds.v[wave][buf]);
     };
     int j = j_a + wave;
     if (j < j_b) fetch(j, 0);
@@ -492,9 +512,9 @@ __global__ void __launch_bounds__(256) window_token_sum_kernel(WindowArgs a, int
   const int unit = (int)(blockIdx.x / kTokenRows), c = (int)(blockIdx.x % kTokenRows);
   const int grp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
   const int group = unit % a.nqt, bh = unit / a.nqt, hk = bh % a.Hkv, b = bh / a.Hkv;
-  const int col = group * kTokenRows + c;
-  if (col >= a.rep * a.Sq) return;
-  const int h = hk * a.rep + token_head(a, col), row = token_row(a, col);
+  const TokenColumn tc = token_column(a, group, c);
+  if (tc.row >= a.Sq) return;
+  const int h = hk * a.rep + tc.head, row = tc.row;
   const float *ml = a.part + (int64_t)units * a.pieces * kTokenRows * 128;
   const int64_t slot = (int64_t)unit * a.pieces * kTokenRows + c;
   float2 x[kPer];
@@ -570,8 +590,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     vdma.init(a.vss, wave, lane);
     auto fetch = [&](int j, auto par) __attribute__((always_inline)) {
       constexpr int P = decltype(par)::value;
-      kdma.issue(Kb, a.kss, st.key0(j), st.limit(j), kbuf[P]);
-      vdma.issue(Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
+      fetch_tile(kdma, Kb, a.kss, st.key0(j), st.limit(j), kbuf[P]);
+      fetch_tile(vdma, Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
     };
     fetch(0, C<0>{});
     u32x4 qf[8], df[8];
@@ -689,13 +709,13 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
     int crow = frow;  // rows of the stage that is computed
     auto fetch = [&](auto par) __attribute__((always_inline)) {
       constexpr int slot = decltype(par)::value;
-      qdma.issue(a.q + it.b * a.qsb + fh * a.qsh, a.qss, frow, i_b, lds.q[slot]);
-      ddma.issue(a.dout + it.b * a.gsb + fh * a.gsh, a.gss, frow, i_b, lds.dout[slot]);
+      fetch_tile(qdma, a.q + it.b * a.qsb + fh * a.qsh, a.qss, frow, i_b, lds.q[slot]);
+      fetch_tile(ddma, a.dout + it.b * a.gsb + fh * a.gsh, a.gss, frow, i_b, lds.dout[slot]);
       // Rows past i_b are zeros throughout: p = 1, but dO = dP = delta = 0.
       if (wave < (kDk ? 2 : 1)) {
         const int rows = i_b - frow < kQStage ? i_b - frow : kQStage;
         const float *st = a.stats + wave * a.stats_n + ((int64_t)it.b * a.H + fh) * a.Sq + frow;
-        buffer_load_lds_b32(range_desc(st, rows * 4), 4 * lane, lds_address(lds.stats[slot][wave]));
+        buffer_load_lds_b32(settled(range_desc(st, rows * 4)), 4 * lane, lds_address(lds.stats[slot][wave]));
       }
       frow += kQStage;
       if (frow >= i_b) {
@@ -865,16 +885,20 @@ size_t window_bwd_bytes(WindowArgs a) {
   return 2 * stat_rows(a) * sizeof(float) + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
 }
 
+// Runs the tiles are dealt in at least: fewer, longer ones share more of their keys in an
+// XCD's L2 (H=56 S=42120, 4096 keys to either side, forward: 10.0 ms in runs of 16 tiles,
+// 9.2 in runs of 64), more of them level the XCDs' work.
+constexpr int kRowRuns = 256, kKeyRuns = 128;
 // Grid of `tiles` work items for each of `heads` heads (item_of), in `runs` runs or more.
 static int deal(int tiles, int heads, int runs_wanted, int *chunk) {
   const int64_t total = (int64_t)heads * tiles, most = total / runs_wanted;
-  *chunk = most < 1 ? 1 : (most > 16 ? 16 : (int)most);
+  *chunk = most < 1 ? 1 : (most > 64 ? 64 : (int)most);
   const int64_t runs = (int64_t)heads * ((tiles + *chunk - 1) / *chunk);
   return (int)((runs + 7) / 8 * 8 * *chunk);
 }
 
 // Query rows up to which splitting the keys is weighed against the tiles.
-constexpr int kTokenMaxRows = 256;
+constexpr int kTokenMaxRows = 1024;
 
 // Whether the keys are split, and into how many workgroups per 32 rows.  In units of a
 // token workgroup's step (four waves' stages of 32 keys, about 2 us of its CU): a round of
@@ -882,13 +906,16 @@ constexpr int kTokenMaxRows = 256;
 // tiles 0.7 (two workgroups to a CU).
 static bool plan_token(WindowArgs &a, int cus) {
   if (a.Sq > kTokenMaxRows) return false;
-  a.nqt = (a.rep * a.Sq + kTokenRows - 1) / kTokenRows;
+  const int per_head = (a.Sq + kTokenRows - 1) / kTokenRows;
+  a.nqt = a.Sq >= kTokenRows ? a.rep * per_head : (a.rep * a.Sq + kTokenRows - 1) / kTokenRows;
   const int64_t units = (int64_t)a.B * a.Hkv * a.nqt;
-  const int64_t range = (int64_t)a.left + a.right + a.Sq < a.Skv ? (int64_t)a.left + a.right + a.Sq : a.Skv;
-  const int64_t keys = range + a.sinks < a.Skv ? range + a.sinks : a.Skv;
-  const int64_t steps = (keys + 4 * kTokenStage - 1) / (4 * kTokenStage);
+  auto keys_of = [&](int rows) -> int64_t {  // of a workgroup with so many rows
+    const int64_t n = (int64_t)a.left + a.right + a.sinks + (rows < a.Sq ? rows : a.Sq);
+    return n < a.Skv ? n : a.Skv;
+  };
+  const int64_t steps = (keys_of(kTokenRows) + 4 * kTokenStage - 1) / (4 * kTokenStage);
   const int64_t tiles = (int64_t)a.B * a.H * ((a.Sq + kRows - 1) / kRows);
-  int64_t best = (tiles + 2 * cus - 1) / (2 * cus) * ((keys + kBN - 1) / kBN) * 7 / 10 + 3;
+  int64_t best = (tiles + 2 * cus - 1) / (2 * cus) * ((keys_of(kRows) + kBN - 1) / kBN) * 7 / 10 + 3;
   a.pieces = 0;
   for (int p = 1; p <= kTokenPieces && p <= steps; ++p) {
     const int64_t rounds = (units * p + cus - 1) / cus;
@@ -925,7 +952,7 @@ int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
   if (rc) return rc;
   if (!plan_token(a, cus)) {
     a.nqt = (a.Sq + kRows - 1) / kRows;
-    const int grid = deal(a.nqt, a.B * a.H, 512, &a.chunk);
+    const int grid = deal(a.nqt, a.B * a.H, kRowRuns, &a.chunk);
     hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
     return check_launch("window_fwd_kernel");
   }
@@ -938,12 +965,11 @@ int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
   return check_launch("window_token_sum_kernel");
 }
 
-constexpr int kKeyRuns = 128;
 int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {
   a.stats = static_cast<float *>(ws);
   a.stats_n = (int64_t)stat_rows(a);
   a.nqt = (a.Sq + kRows - 1) / kRows;
-  const int grid = deal(a.nqt, a.B * a.H, 512, &a.chunk);
+  const int grid = deal(a.nqt, a.B * a.H, kRowRuns, &a.chunk);
   hipLaunchKernelGGL(window_dq_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   int rc = check_launch("window_dq_kernel");
   if (rc) return rc;

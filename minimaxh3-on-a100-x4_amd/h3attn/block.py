@@ -50,20 +50,26 @@ def _rope_weight(name: str, w: torch.Tensor, device) -> torch.Tensor:
     return w
 
 
-def _positions(pos: torch.Tensor, axes, theta, B: int, S: int, device):
-    axes = tuple(int(d) for d in axes)
+@functools.lru_cache(maxsize=256)
+def _axes_dims(axes: tuple):
+    """Checked rotated dims of each axis as the entry points take them."""
     if not 1 <= len(axes) <= _lib.MAX_AXES:
         raise ValueError(f"axes must name the rotated dims of 1 to {_lib.MAX_AXES} axes, got {axes}")
-    if any(d <= 0 or d % 2 for d in axes) or sum(axes) > HEAD_DIM or sum(axes) % 16:
+    if any(d != int(d) or d <= 0 or d % 2 for d in axes) or sum(axes) > HEAD_DIM or sum(axes) % 16:
         raise ValueError(f"axes {axes}: even dims that add up to a multiple of 16, at most {HEAD_DIM}")
+    return (ctypes.c_int * _lib.MAX_AXES)(*(int(d) for d in axes))
+
+
+def _positions(pos: torch.Tensor, axes, theta, B: int, S: int, device):
+    axes = tuple(axes)
+    dims, A, shape = _axes_dims(axes), len(axes), pos.shape
     if pos.dtype not in (torch.int32, torch.float32) or pos.device != device:
         raise ValueError(f"positions must be int32 or float32 on q's device, got {pos.dtype} on {pos.device}")
-    if tuple(pos.shape) not in ((S, len(axes)), (1, S, len(axes)), (B, S, len(axes))):
-        raise ValueError(f"positions {tuple(pos.shape)} must be [S, axes] or [B, S, axes] (B={B}, S={S}, axes {axes})")
+    if shape[-2:] != (S, A) or len(shape) > 3 or (len(shape) == 3 and shape[0] not in (1, B)):
+        raise ValueError(f"positions {tuple(shape)} must be [S, axes] or [B, S, axes] (B={B}, S={S}, axes {axes})")
     pos = pos.contiguous()
-    stride = S * len(axes) if pos.dim() == 3 and pos.shape[0] == B else 0
-    dims = (ctypes.c_int * _lib.MAX_AXES)(*axes)
-    return pos, _lib.Positions(pos.data_ptr(), stride, int(pos.dtype == torch.float32), len(axes), dims, float(theta))
+    stride = S * A if len(shape) == 3 and shape[0] == B else 0
+    return pos, _lib.Positions(pos.data_ptr(), stride, 1 if pos.dtype == torch.float32 else 0, A, dims, float(theta))
 
 
 def _rope_prepare(q, k, pos, axes, qw, kw, theta):
@@ -133,8 +139,21 @@ def qk_rmsnorm_rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor
 # ---------------------------------------------------------------------------
 # layer norm
 @functools.lru_cache(maxsize=256)
-def _bounds(segments: tuple):
-    return (ctypes.c_int * len(segments))(*segments)
+def _bounds(segments, rows: int, groups):
+    """Checked bounds of the segments as the entry points take them; None: `groups` equal ones."""
+    if rows > 2 ** 31 - 1:
+        raise ValueError("too many rows")
+    if segments is None:
+        groups = groups or 1
+        if rows % groups:
+            raise ValueError(f"{rows} rows do not split evenly into {groups} segments: pass their bounds")
+        segments = tuple(i * (rows // groups) for i in range(groups + 1))
+    if len(segments) < 2 or segments[0] != 0 or segments[-1] != rows or \
+            any(b < a for a, b in zip(segments, segments[1:])):
+        raise ValueError(f"segments must be non-decreasing bounds from 0 to {rows} rows, got {segments}")
+    if groups is not None and groups != len(segments) - 1:
+        raise ValueError(f"{len(segments) - 1} segments, but weights for {groups}")
+    return (ctypes.c_int * len(segments))(*(int(b) for b in segments))
 
 
 def _norm_rows(name: str, t: torch.Tensor, C: int) -> torch.Tensor:
@@ -167,23 +186,10 @@ def _norm_prepare(x, weight, bias, segments):
         if groups is not None and n != groups:
             raise ValueError("weight and bias must have the same segments")
         groups = n
-    if segments is None:
-        groups = groups or 1
-        if rows % groups:
-            raise ValueError(f"{rows} rows do not split evenly into {groups} segments: pass their bounds")
-        segments = tuple(i * (rows // groups) for i in range(groups + 1))
-    else:
-        segments = tuple(int(b) for b in segments)
-        if len(segments) < 2 or segments[0] != 0 or segments[-1] != rows or \
-                any(b < a for a, b in zip(segments, segments[1:])):
-            raise ValueError(f"segments must be non-decreasing bounds from 0 to {rows} rows, got {segments}")
-        if groups is not None and groups != len(segments) - 1:
-            raise ValueError(f"{len(segments) - 1} segments, but weights for {groups}")
-    if rows > 2 ** 31 - 1:
-        raise ValueError("too many rows")
+    bounds = _bounds(None if segments is None else tuple(segments), rows, groups)
     dt = DTYPES[affine[0][1].dtype] if affine else _lib.FP32
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    return rows, C, segments, dt, weight, bias
+    return rows, C, bounds, dt, weight, bias
 
 
 def _ptr(t):
@@ -201,14 +207,14 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     16384; weight and bias any of these.  Returns y, with return_stats (y, mean, rstd),
     the fp32 [rows] statistics that layer_norm_bwd takes.
     """
-    rows, C, segments, dt, weight, bias = _norm_prepare(x, weight, bias, segments)
+    rows, C, bounds, dt, weight, bias = _norm_prepare(x, weight, bias, segments)
     x2 = _norm_rows("x", x, C)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
     with _on_device(x):
         rc = lib().h3a_layer_norm_fwd(x2.data_ptr(), x2.stride(0), _ptr(weight), _ptr(bias), y.data_ptr(), C,
                                       _ptr(stats), None if stats is None else stats[1].data_ptr(), rows, C,
-                                      DTYPES[x.dtype], dt, _bounds(segments), len(segments) - 1, int(modulate),
+                                      DTYPES[x.dtype], dt, bounds, len(bounds) - 1, 1 if modulate else 0,
                                       float(eps), _stream(x))
     check("h3a_layer_norm_fwd", rc)
     return (y, stats[0], stats[1]) if return_stats else y
@@ -222,7 +228,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
     a fixed order, [C], or [n, C] where weight is or segments are given; None without
     param_grads.
     """
-    rows, C, segments, dt, weight, _ = _norm_prepare(x, weight, None, segments)
+    rows, C, bounds, dt, weight, _ = _norm_prepare(x, weight, None, segments)
     if not isinstance(dy, torch.Tensor) or dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("dy must be a tensor like x")
     for name, t in (("mean", mean), ("rstd", rstd)):
@@ -230,18 +236,18 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
             raise ValueError(f"{name} must be the forward's fp32 [{rows}] statistics")
     x2, dy2 = _norm_rows("x", x, C), _norm_rows("dy", dy, C)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = len(segments) - 1
+    n = len(bounds) - 1
     grads, ws, nbytes = None, None, ctypes.c_size_t(0)
     with _on_device(x):
         if param_grads:
             grads = torch.empty((2, n, C), dtype=torch.float32, device=x.device)
             check("h3a_layer_norm_bwd_workspace_size",
-                  lib().h3a_layer_norm_bwd_workspace_size(_bounds(segments), n, C, ctypes.byref(nbytes)))
+                  lib().h3a_layer_norm_bwd_workspace_size(bounds, n, C, ctypes.byref(nbytes)))
             ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
         rc = lib().h3a_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(weight),
                                       mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), C, _ptr(grads),
                                       None if grads is None else grads[1].data_ptr(), rows, C, DTYPES[x.dtype], dt,
-                                      _bounds(segments), n, int(modulate), _ptr(ws), nbytes.value, _stream(x))
+                                      bounds, n, 1 if modulate else 0, _ptr(ws), nbytes.value, _stream(x))
     check("h3a_layer_norm_bwd", rc)
     if grads is None:
         return dx, None, None

@@ -8,6 +8,7 @@ wraps both in a differentiable function.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -18,7 +19,7 @@ from .ops import HEAD_DIM, _as_kernel_input, _layout, _on_device, _stream
 
 
 # Query rows up to which the forward may split the keys, and need a workspace.
-SPLIT_ROWS = 256
+SPLIT_ROWS = 1024
 
 
 def _side(name: str, n) -> int:
@@ -37,27 +38,44 @@ def _per_sequence(name: str, t: torch.Tensor, B: int, device) -> int:
     return t.data_ptr()
 
 
-def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device) -> _lib.Window:
-    try:
-        left, right = window
-    except TypeError:
-        raise ValueError(f"window must be a pair (left, right), got {window!r}") from None
-    left, right = _side("window's left side", left), _side("window's right side", right)
+@functools.lru_cache(maxsize=1024)
+def _sides(window, sinks, causal, start, Sq, Skv):
+    """(left, right, sinks, causal, start) of a checked window; start None: given per sequence."""
+    if not isinstance(window, tuple) or len(window) != 2:
+        raise ValueError(f"window must be a pair (left, right), got {window!r}")
+    left, right = _side("window's left side", window[0]), _side("window's right side", window[1])
     if causal and window[1] not in (0, None):
         raise ValueError(f"a causal window has no right side, got {window[1]}")
-    lens = None if kv_lens is None else _per_sequence("kv_lens", kv_lens, B, device)
-    start, starts = 0, None
-    if isinstance(q_start, torch.Tensor):
-        starts = _per_sequence("q_start", q_start, B, device)
-    elif q_start is None:
-        if lens is not None and Sq != Skv:
-            raise ValueError("kv_lens with Sq != Skv needs q_start: where the queries sit in the sequences")
-        start = Skv - Sq
-    else:
-        start = int(q_start)
-    if starts is None and not 0 <= start <= Skv - Sq:
+    if start is not None and not 0 <= start <= Skv - Sq:
         raise ValueError(f"q_start {start}: rows must lie at positions 0 .. Skv - 1 (Sq={Sq}, Skv={Skv})")
-    return _lib.Window(left, right, _side("sinks", sinks), 1 if causal else 0, start, starts, lens)
+    return left, right, _side("sinks", sinks), 1 if causal else 0, 0 if start is None else start
+
+
+def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device):
+    """The call's h3a_window, and what its workspace's size depends on."""
+    if isinstance(window, list):
+        window = tuple(window)
+    lens = None if kv_lens is None else _per_sequence("kv_lens", kv_lens, B, device)
+    starts = None
+    if isinstance(q_start, torch.Tensor):
+        starts, start = _per_sequence("q_start", q_start, B, device), None
+    elif q_start is not None:
+        start = int(q_start)
+    elif lens is not None and Sq != Skv:
+        raise ValueError("kv_lens with Sq != Skv needs q_start: where the queries sit in the sequences")
+    else:
+        start = Skv - Sq
+    sides = _sides(window, sinks, bool(causal), start, Sq, Skv)
+    return _lib.Window(*sides, starts, lens), sides
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(fn: str, sizes: tuple, sides: tuple, device_index: int) -> int:
+    """Workspace bytes of entry point fn on the device, which is the current one."""
+    left, right, sinks, causal, start = sides
+    w, n = _lib.Window(left, right, sinks, causal, 0, None, None), ctypes.c_size_t(0)
+    check(fn, getattr(lib(), fn)(*sizes, ctypes.byref(w), ctypes.byref(n)))
+    return n.value
 
 
 def _prepare(q, k, v):
@@ -97,7 +115,7 @@ def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, s
     attn_bwd_window takes.  Strides and `out` as for attn_fwd.
     """
     q, k, v, (B, H, Hkv, Sq, Skv, D), st = _prepare(q, k, v)
-    w = _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, q.device)
+    w, sides = _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, q.device)
     if out is None:
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
         ost = out.stride()[:3]
@@ -111,10 +129,8 @@ def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, s
     with _on_device(q):
         ws, nbytes = None, 0
         if Sq <= SPLIT_ROWS:
-            n = ctypes.c_size_t(0)
-            check("h3a_attn_fwd_window_workspace_size",
-                  lib().h3a_attn_fwd_window_workspace_size(B, H, Hkv, Sq, Skv, D, ctypes.byref(w), ctypes.byref(n)))
-            nbytes = n.value
+            nbytes = _workspace_bytes("h3a_attn_fwd_window_workspace_size", (B, H, Hkv, Sq, Skv, D), sides,
+                                      q.get_device())
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib().h3a_attn_fwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                        None if lse is None else lse.data_ptr(), B, H, Hkv, Sq, Skv, D, *st,
@@ -149,17 +165,15 @@ def attn_bwd_window(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     o, ost = _as_kernel_input("o", o)
     if lse.shape != (B, H, Sq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise ValueError(f"lse must be the forward's fp32 [{B},{H},{Sq}] tensor")
-    w = _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, q.device)
+    w, sides = _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, q.device)
     (dq, dqst), (dk, dkst), (dv, dvst) = _grad_like(q), _grad_like(k), _grad_like(v)
     sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
     with _on_device(q):
-        n = ctypes.c_size_t(0)
-        check("h3a_attn_bwd_window_workspace_size",
-              lib().h3a_attn_bwd_window_workspace_size(B, H, Hkv, Sq, Skv, D, ctypes.byref(w), ctypes.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        nbytes = _workspace_bytes("h3a_attn_bwd_window_workspace_size", (B, H, Hkv, Sq, Skv, D), sides, q.get_device())
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib().h3a_attn_bwd_window(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                        lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Sq,
                                        Skv, D, gst, *st, ost, dqst, dkst, dvst, ctypes.byref(w), sc, ws.data_ptr(),
-                                       n.value, _stream(q))
+                                       nbytes, _stream(q))
     check("h3a_attn_bwd_window", rc)
     return dq, dk, dv
