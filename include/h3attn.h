@@ -248,7 +248,7 @@ typedef struct {
  * exp(scale * q.k) over the keys seen, for h3a_attn_bwd_window.  Strides and
  * alignment as h3a_attn_fwd, and every sequence stride < 2^24 elements; lengths
  * up to 2^29.  workspace: h3a_attn_fwd_window_workspace_size bytes for the current
- * device (0, so NULL, for more than 1024 rows: fewer may be split along the keys),
+ * device (0, so NULL, for more than 8192 rows: fewer may be split along the keys),
  * untouched until the call's work has completed.  No counterpart in the reference.
  */
 int h3a_attn_fwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D,

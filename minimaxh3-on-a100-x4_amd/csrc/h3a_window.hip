@@ -170,9 +170,11 @@ __device__ __forceinline__ void load_columns(u32x4 (&f)[8], const uint16_t *base
 
 // acc * mul, rounded to bf16, to rows row0 .. row0 + nrows - 1: through a wave-private
 // LDS tile, so that every store writes four whole rows.  Columns whose `live` is false
-// store zeros.
+// store zeros; patch(put) may replace rows: put(row, a, b) sets the lane's dims 2*lane and
+// 2*lane + 1.
+template <class Patch>
 __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul, bool live, uint8_t *tile,
-                                              uint16_t *base, int64_t stride, int nrows, int lane) {
+                                              uint16_t *base, int64_t stride, int nrows, int lane, Patch patch) {
   const int g = lane >> 5, l32 = lane & 31;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) {
@@ -185,6 +187,9 @@ __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul,
       *(u32x2 *)(tile + l32 * 256 + ((c ^ (l32 & 15)) << 4) + 8 * g) = val;
     }
   }
+  patch([&](int row, float x, float y) __attribute__((always_inline)) {
+    *(uint32_t *)(tile + row * 256 + (((lane >> 2) ^ (row & 15)) << 4) + 4 * (lane & 3)) = pack_bf16x2(x, y);
+  });
   const int ch = lane & 15;
   const __amdgpu_buffer_rsrc_t res = stage_rsrc(base, stride, nrows < 32 ? nrows : 32);
 #pragma unroll
@@ -193,6 +198,57 @@ __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul,
     const u32x4 val = *(const u32x4 *)(tile + r * 256 + ((ch ^ (r & 15)) << 4));
     __builtin_amdgcn_raw_buffer_store_b128(val, res, (int)((uint32_t)r * (uint32_t)stride * 2u + 16u * ch), 0, 0);
   }
+}
+
+// The kernels' products multiply a hidden pair's weight, 0, with what the hidden row holds,
+// which is not 0 where that is an infinity or NaN.  So a column whose sum is not finite is
+// taken again by its wave from the pairs that see each other alone: rare, and slow.
+
+// Columns (bit c: column c) of a wave's accumulators that hold a value that is not finite.
+__device__ __forceinline__ uint32_t spoiled_columns(const f32x16 (&acc)[4], bool counts) {
+  bool bad = false;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bad |= (__float_as_uint(acc[dt][r]) & 0x7f800000u) == 0x7f800000u;
+  const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad && counts);
+  return (uint32_t)(lanes | lanes >> 32);
+}
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// Natural logarithm of l * 2^m: -inf for an empty sum, l where that is not finite.
+__device__ __forceinline__ float log_sum(float m, float l) {
+  return !finite(l) ? l : (l > 0.f ? (m + log2f(l)) * kLn2 : kNegInf);
+}
+
+__device__ __forceinline__ float dot128(const uint16_t *x, const uint16_t *y) {
+  float sum = 0.f;
+  for (int d = 0; d < 128; d += 8) {
+    const u32x4 a = *(const u32x4 *)(x + d), b = *(const u32x4 *)(y + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fmaf(bf16_hi(a[i]), bf16_hi(b[i]), fmaf(bf16_lo(a[i]), bf16_lo(b[i]), sum));
+  }
+  return sum;
+}
+
+// acc (the lane's dims 2*lane, 2*lane + 1) += sum over rows row0 .. row0 + 63 below limit of
+// weight(row) * Y[row], over the rows for which sees(row).
+template <class Sees, class Weight>
+__device__ __forceinline__ void add_seen_rows(float2 &acc, int row0, int limit, const uint16_t *Y, int64_t stride, int lane,
+                                              Sees sees, Weight weight) {
+  const int row = row0 + lane;
+  const bool seen = row < limit && sees(row);
+  const float w = seen ? weight(row) : 0.f;
+  for (uint64_t left = __builtin_amdgcn_ballot_w64(seen); left; left &= left - 1) {
+    const int i = __builtin_ctzll(left);
+    const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
+    const uint32_t y = *(const uint32_t *)(Y + (int64_t)(row0 + i) * stride + 2 * lane);
+    acc.x = fmaf(wi, bf16_lo(y), acc.x);
+    acc.y = fmaf(wi, bf16_hi(y), acc.y);
+  }
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
 // DMA of the rows of [row0, limit) that a tile holds, the rest as zeros.
@@ -298,6 +354,20 @@ __device__ __forceinline__ Item item_of(const WindowArgs &a, int i, int chunk, i
   return {bh < a.B * heads && tile < tiles ? tile : -1, bh % heads, bh / heads};
 }
 
+// add_seen_rows over all keys that position pos sees: weights weight(key, its row of K),
+// rows of Y.
+template <class Weight>
+__device__ __forceinline__ void each_seen_key(const WindowArgs &a, const Span &sp, int pos, const uint16_t *K,
+                                              const uint16_t *Y, int64_t ystride, int lane, float2 &sum,
+                                              Weight weight) {
+  KeyStages<> st;
+  st.init(a, sp, pos, pos);
+  for (int j = 0; j < st.n; ++j)
+    add_seen_rows(
+        sum, st.key0(j), st.limit(j), Y, ystride, lane, [](int) { return true; },
+        [&](int key) { return weight(key, K + (int64_t)key * a.kss); });
+}
+
 // Forward.  A workgroup takes 128 query rows of one head, a wave 32 of them; the
 // 64-key stages of their window are double-buffered in LDS by DMA, two workgroups to a
 // CU, so that one's softmax overlaps the other's MFMAs.
@@ -359,10 +429,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const float ltot = half_swap_sum(lsum);
   const float inv = ltot > 0.f ? 1.f / ltot : 0.f;
   if (a.lse && g == 0 && row < a.Sq)
-    a.lse[((int64_t)it.b * a.H + it.h) * a.Sq + row] = live && ltot > 0.f ? (m + log2f(ltot)) * kLn2 : kNegInf;
+    a.lse[((int64_t)it.b * a.H + it.h) * a.Sq + row] = live ? log_sum(m, ltot) : kNegInf;
   if (wq0 < a.Sq)
     store_columns(o, inv, live, reinterpret_cast<uint8_t *>(&kbuf[0][0]) + wave * 8192,
-                  a.o + it.b * a.osb + it.h * a.osh + (int64_t)wq0 * a.oss, a.oss, a.Sq - wq0, lane);
+                  a.o + it.b * a.osb + it.h * a.osh + (int64_t)wq0 * a.oss, a.oss, a.Sq - wq0, lane,
+                  [&](auto put) __attribute__((always_inline)) {
+                    for (uint32_t left = spoiled_columns(o, live && finite(ltot)); left; left &= left - 1) {
+                      const int c = __builtin_ctz(left), r = wq0 + c;
+                      const float mc = lane_value(m, c), ic = lane_value(inv, c);
+                      const uint16_t *q = a.q + it.b * a.qsb + it.h * a.qsh + (int64_t)r * a.qss;
+                      float2 sum = {0.f, 0.f};
+                      each_seen_key(a, sp, sp.qs + r, Kb, Vb, a.vss, lane, sum, [&](int, const uint16_t *k) {
+                        return fast_exp2(fmaf(dot128(q, k), a.sl2, -mc));
+                      });
+                      put(c, sum.x * ic, sum.y * ic);
+                    }
+                  });
 }
 
 // Forward for few query rows (a new token, or a short chunk of them, against a cache).
@@ -463,6 +545,33 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) xch[((wave * 4 + dt) * 16 + r) * 64 + lane] = o[dt][r];
+  for (uint32_t left = spoiled_columns(o, live && finite(ltot)); left; left &= left - 1) {
+    const int c = __builtin_ctz(left);
+    const TokenColumn tc = token_column(a, group, c);
+    const int hc = hk * a.rep + tc.head, pc = sp.qs + tc.row;
+    const float mc = lane_value(m, c);
+    const uint16_t *q = a.q + b * a.qsb + hc * a.qsh + (int64_t)tc.row * a.qss;
+    const int lo = pc - a.left, first = first_keys(a, sp, pc);
+    const int hi = pc + a.right < sp.len - 1 ? pc + a.right : sp.len - 1;
+    KeyStages<kTokenStage> st;
+    st.init(a, sp, sp.qs + r0, sp.qs + r1);
+    const int j_a = (int)((int64_t)st.n * piece / a.pieces), j_b = (int)((int64_t)st.n * (piece + 1) / a.pieces);
+    float2 sum = {0.f, 0.f};
+    for (int j = j_a + wave; j < j_b; j += 4) {
+      const int end = st.key0(j) + kTokenStage;
+      add_seen_rows(
+          sum, st.key0(j), end < st.limit(j) ? end : st.limit(j), a.v + b * a.vsb + hk * a.vsh, a.vss, lane,
+          [&](int key) { return (j >= st.n_first && key >= lo && key <= hi) || key < first; },
+          [&](int key) {
+            return fast_exp2(fmaf(dot128(q, a.k + b * a.ksb + hk * a.ksh + (int64_t)key * a.kss), a.sl2, -mc));
+          });
+    }
+    // Dims 2*lane and 2*lane + 1 of column c in the accumulators' order.
+    const int d = 2 * lane, r = 4 * ((d & 31) >> 3) + (d & 3);
+    float *at = xch + ((wave * 4 + (d >> 5)) * 16 + r) * 64 + 32 * ((d >> 2) & 1) + c;
+    at[0] = sum.x;
+    at[64] = sum.y;
+  }
   ml[wave * 64 + lane] = float2{m, ltot};
   __syncthreads();
   float top = kNegInf, l = 0.f, w[4];
@@ -496,7 +605,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
       float *stat = a.part + (int64_t)gridDim.x * kTokenRows * 128 + slot * 2;
       *(float2 *)stat = live ? float2{top, l} : float2{kNegInf, 0.f};
     } else if (a.lse && has) {
-      a.lse[((int64_t)b * a.H + h) * a.Sq + row] = live && l > 0.f ? (top + log2f(l)) * kLn2 : kNegInf;
+      a.lse[((int64_t)b * a.H + h) * a.Sq + row] = live ? log_sum(top, l) : kNegInf;
     }
   }
 }
@@ -555,7 +664,7 @@ __global__ void __launch_bounds__(256) window_token_sum_kernel(WindowArgs a, int
   const float inv = l > 0.f ? 1.f / l : 0.f;
   *(u32x2 *)(a.o + b * a.osb + h * a.osh + row * a.oss + d) =
       u32x2{pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv)};
-  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Sq + row] = l > 0.f ? (top + log2f(l)) * kLn2 : kNegInf;
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Sq + row] = log_sum(top, l);
 }
 
 // Backward, dQ: tiles and stages as forward, with P from the stored lse.  The rows' lse
@@ -576,6 +685,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const uint16_t *Vb = a.v + it.b * a.vsb + (it.h / a.rep) * a.vsh;
 
   f32x16 dq[4];
+  float delta = 0.f, l2 = 0.f;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) dq[dt] = f32x16{0.f};
   if (r1 >= r0) {
@@ -597,7 +707,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     u32x4 qf[8], df[8];
     load_columns(qf, a.q + it.b * a.qsb + it.h * a.qsh, a.qss, row, a.Sq, g);
     load_columns(df, a.dout + it.b * a.gsb + it.h * a.gsh, a.gss, row, a.Sq, g);
-    float delta = 0.f;
     {
       u32x4 of[8];
       load_columns(of, a.o + it.b * a.osb + it.h * a.osh, a.oss, row, a.Sq, g);
@@ -609,7 +718,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       delta = half_swap_sum(delta);
     }
     const int64_t stat = ((int64_t)it.b * a.H + it.h) * a.Sq + (row < a.Sq ? row : a.Sq - 1);
-    const float l2 = a.lse[stat] == kNegInf ? -kNegInf : a.lse[stat] * kLog2e;
+    l2 = a.lse[stat] == kNegInf ? -kNegInf : a.lse[stat] * kLog2e;
     if (g == 0 && row < a.Sq) {
       a.stats[stat] = l2;
       a.stats[a.stats_n + stat] = delta;
@@ -644,7 +753,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   }
   if (wq0 < a.Sq)
     store_columns(dq, a.scale, live, reinterpret_cast<uint8_t *>(&kbuf[0][0]) + wave * 8192,
-                  a.dq + it.b * a.dqsb + it.h * a.dqsh + (int64_t)wq0 * a.dqss, a.dqss, a.Sq - wq0, lane);
+                  a.dq + it.b * a.dqsb + it.h * a.dqsh + (int64_t)wq0 * a.dqss, a.dqss, a.Sq - wq0, lane,
+                  [&](auto put) __attribute__((always_inline)) {
+                    for (uint32_t left = spoiled_columns(dq, live && finite(delta)); left; left &= left - 1) {
+                      const int c = __builtin_ctz(left), r = wq0 + c;
+                      const float lc = lane_value(l2, c), dc = lane_value(delta, c);
+                      const uint16_t *q = a.q + it.b * a.qsb + it.h * a.qsh + (int64_t)r * a.qss;
+                      const uint16_t *d = a.dout + it.b * a.gsb + it.h * a.gsh + (int64_t)r * a.gss;
+                      float2 sum = {0.f, 0.f};
+                      each_seen_key(a, sp, sp.qs + r, Kb, Kb, a.kss, lane, sum, [&](int key, const uint16_t *k) {
+                        return fast_exp2(fmaf(dot128(q, k), a.sl2, -lc)) * (dot128(d, Vb + (int64_t)key * a.vss) - dc);
+                      });
+                      put(c, sum.x * a.scale, sum.y * a.scale);
+                    }
+                  });
 }
 
 // Backward, dK and dV: a workgroup sums one of them over 128 keys of one key head, a wave
@@ -797,21 +919,58 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
       __syncthreads();
     });
   }
+  // Column c of this piece again, from the rows that see it.
+  auto column_again = [&](int c) __attribute__((always_inline)) -> float2 {
+    float2 sum = {0.f, 0.f};
+    const int key_c = wj0 + c, plo_c = key_c < a.sinks ? (a.causal ? key_c : -(1 << 30)) : key_c - a.right;
+    const uint32_t span_c = key_c < a.sinks ? 0x7fffffffu : (uint32_t)(a.left + a.right);
+    const uint16_t *k = a.k + it.b * a.ksb + it.h * a.ksh + (int64_t)key_c * a.kss;
+    const uint16_t *v = a.v + it.b * a.vsb + it.h * a.vsh + (int64_t)key_c * a.vss;
+    for (int64_t t = t_a; t < t_a + n; ++t) {
+      const int h = it.h * a.rep + (int)(t / per_head), row0 = i_a + (int)(t % per_head) * kQStage;
+      const uint16_t *q = a.q + it.b * a.qsb + h * a.qsh, *d = a.dout + it.b * a.gsb + h * a.gsh;
+      const float *st = a.stats + ((int64_t)it.b * a.H + h) * a.Sq;
+      add_seen_rows(
+          sum, row0, i_b, kDk ? q : d, kDk ? a.qss : a.gss, lane,
+          [&](int row) { return (uint32_t)(sp.qs + row - plo_c) <= span_c; },
+          [&](int row) {
+            const float p = fast_exp2(fmaf(dot128(q + (int64_t)row * a.qss, k), a.sl2, -st[row]));
+            return kDk ? p * (dot128(d + (int64_t)row * a.gss, v) - st[a.stats_n + row]) : p;
+          });
+    }
+    return sum;
+  };
+  const uint32_t spoiled = n > 0 ? spoiled_columns(acc, key < sp.len) : 0;
   if (piece >= 0) {
     const int64_t bh = (int64_t)it.b * a.Hkv + it.h;
     float *part = a.part + (((bh * a.first_tiles + it.tile) * a.pieces + piece) * 2 + (kDk ? 0 : 1)) * (kRows * 128) +
-                  (32 * wave + l32) * 128 + 4 * g;
+                  32 * wave * 128;
+    if (!(spoiled >> l32 & 1)) {
+      float *p = part + l32 * 128 + 4 * g;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+      for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int rr = 0; rr < 4; ++rr)
-        *(float4 *)(part + dt * 32 + 8 * rr) =
-            float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]};
+        for (int rr = 0; rr < 4; ++rr)
+          *(float4 *)(p + dt * 32 + 8 * rr) =
+              float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]};
+    }
+    for (uint32_t left = spoiled; left; left &= left - 1) {
+      const int c = __builtin_ctz(left);
+      *(float2 *)(part + c * 128 + 2 * lane) = column_again(c);
+    }
   } else if (wj0 < a.Skv) {
     uint8_t *tile = reinterpret_cast<uint8_t *>(&lds.q[0][0]) + wave * 8192;
     uint16_t *out = kDk ? a.dk + it.b * a.dksb + it.h * a.dksh + (int64_t)wj0 * a.dkss
                         : a.dv + it.b * a.dvsb + it.h * a.dvsh + (int64_t)wj0 * a.dvss;
-    store_columns(acc, kDk ? a.scale : 1.f, key < sp.len, tile, out, kDk ? a.dkss : a.dvss, a.Skv - wj0, lane);
+    const float mul = kDk ? a.scale : 1.f;
+    store_columns(acc, mul, key < sp.len, tile, out, kDk ? a.dkss : a.dvss, a.Skv - wj0, lane,
+                  [&](auto put) __attribute__((always_inline)) {
+                    for (uint32_t left = spoiled; left; left &= left - 1) {
+                      const int c = __builtin_ctz(left);
+                      const float2 sum = column_again(c);
+                      put(c, sum.x * mul, sum.y * mul);
+                    }
+                  });
   }
 }
 
@@ -898,7 +1057,7 @@ static int deal(int tiles, int heads, int runs_wanted, int *chunk) {
 }
 
 // Query rows up to which splitting the keys is weighed against the tiles.
-constexpr int kTokenMaxRows = 1024;
+constexpr int kTokenMaxRows = 8192;
 
 // Whether the keys are split, and into how many workgroups per 32 rows.  In units of a
 // token workgroup's step (four waves' stages of 32 keys, about 2 us of its CU): a round of

@@ -19,7 +19,7 @@ from .ops import HEAD_DIM, _as_kernel_input, _layout, _on_device, _stream
 
 
 # Query rows up to which the forward may split the keys, and need a workspace.
-SPLIT_ROWS = 1024
+SPLIT_ROWS = 8192
 
 
 def _side(name: str, n) -> int:

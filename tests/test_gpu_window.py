@@ -82,6 +82,77 @@ def test_padded_batch(gpu, causal):
     check(gpu, len(lens), 2, 1, 260, 260, (40, 0 if causal else 40), 6, causal, kv_lens=lens)
 
 
+@pytest.mark.parametrize("S,window,sinks,causal", [(129, (30, 30), 5, False), (257, (0, 64), 0, False),
+                                                   (300, (100, 0), 70, True), (300, (None, None), 0, False)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_many_heads(gpu, S, window, sinks, causal, ragged):
+    """Launches of more tiles than a split of the keys is worth."""
+    lens = [S, 1, S // 2, S - 1] if ragged else None
+    check(gpu, 4, 40, 8, S, S, window, sinks, causal, kv_lens=lens, seed=S)
+
+
+@pytest.mark.parametrize("B,H,Hkv,S,window,sinks", [(1, 2, 1, 200, (20, 20), 3), (1, 1, 1, 700, (40, 30), 130),
+                                                    (4, 40, 8, 200, (20, 20), 3)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("where", ["kv", "q"])
+def test_hidden_values_do_not_matter(gpu, B, H, Hkv, S, window, sinks, bad, where):
+    """NaN and infinities in rows of k and v, or of q and dout, reach those who see them and nobody else."""
+    q, k, v, do = make(gpu, B, H, Hkv, S, S, 4)
+    mask = ref.visible(B, S, S, window, sinks, False, None, None)
+    c = [t.cpu() for t in (q, k, v, do)]
+    spots = [sinks + 5, S // 2, S - 1]
+    if where == "kv":
+        for n, t in enumerate((k, v)):
+            t[:, :, spots[n:]] = bad
+        rows = mask[:, :, spots].any(-1)        # rows that see a bad key
+    else:
+        for n, t in enumerate((q, do)):
+            t[:, :, spots[n:]] = bad
+        rows = torch.zeros(B, S, dtype=torch.bool)
+        rows[:, spots] = True
+    keys = (mask & rows[:, :, None]).any(1)     # keys seen by such rows
+    if where == "kv":
+        keys[:, spots] = True
+    kw = dict(window=window, sinks=sinks)
+    o, lse = h3attn.attn_fwd_window(q, k, v, return_lse=True, **kw)
+    grads = h3attn.attn_bwd_window(do, q, k, v, o, lse, **kw)
+    for name, got, want, bound, hit in zip(
+            ("O", "dq", "dk", "dv"), (o, *grads),
+            (ref.forward(*c[:3], mask, SCALE)[0], *ref.backward(c[3], *c[:3], mask, SCALE)),
+            (ref.forward_bound(*c[:3], mask, SCALE), *ref.backward_bounds(c[3], *c[:3], mask, SCALE)),
+            (rows, rows, keys, keys)):
+        clean = ~hit[:, None, :].expand(*got.shape[:3])
+        assert clean.any()
+        close(got.cpu()[clean], want[clean], bound[clean], name)
+    if bad != bad:
+        assert torch.isnan(o.cpu().float()).any(-1)[rows[:, None].expand(B, H, S)].any()
+
+
+def test_padding_holds_anything(gpu):
+    """Rows and keys behind a sequence's end are NaN: outputs are 0 there and right elsewhere."""
+    B, H, Hkv, S = 3, 4, 2, 190
+    q, k, v, do = make(gpu, B, H, Hkv, S, S, 8)
+    lens = [190, 70, 0]
+    mask = ref.visible(B, S, S, (25, 25), 9, False, None, lens)
+    c = [t.cpu() for t in (q, k, v, do)]
+    for t in (q, k, v, do):
+        for b, n in enumerate(lens):
+            t[b, :, n:] = float("nan")
+    kw = dict(window=(25, 25), sinks=9, kv_lens=torch.tensor(lens, dtype=torch.int32, device=gpu))
+    o, lse = h3attn.attn_fwd_window(q, k, v, return_lse=True, **kw)
+    close(o, ref.forward(*c[:3], mask, SCALE)[0], ref.forward_bound(*c[:3], mask, SCALE), "O")
+    for name, g, w, b in zip(("dq", "dk", "dv"), h3attn.attn_bwd_window(do, q, k, v, o, lse, **kw),
+                             ref.backward(c[3], *c[:3], mask, SCALE), ref.backward_bounds(c[3], *c[:3], mask, SCALE)):
+        close(g, w, b, name)
+    # One token: nothing past its length is read.
+    n = torch.tensor([190, 70, 1], dtype=torch.int32, device=gpu)
+    got = h3attn.attn_fwd_window(c[0][:, :, :1].to(gpu), k, v, (60, 0), sinks=4, causal=True, q_start=n - 1, kv_lens=n)
+    mask = ref.visible(B, 1, S, (60, 0), 4, True, [189, 69, 0], [190, 70, 1])
+    assert torch.isfinite(got[:2]).all()
+    want = ref.forward(c[0][:, :, :1], *c[1:3], mask, SCALE)[0]
+    close(got[:2], want[:2], ref.forward_bound(c[0][:, :, :1], *c[1:3], mask, SCALE)[:2], "one token")
+
+
 @pytest.mark.parametrize("Sq,Skv,q_start", [(1, 300, None), (5, 300, None), (5, 300, 0), (130, 300, 100), (64, 65, 1)])
 def test_chunk_of_queries(gpu, Sq, Skv, q_start):
     check(gpu, 1, 4, 2, Sq, Skv, (70, 0), 5, True, q_start=q_start)

@@ -54,7 +54,7 @@ def test_workspace_refusals():
     assert size(1, 2, 1, 40, 40, 128, None, ctypes.byref(n)) == _lib.H3A_ERR_INVALID_ARG
     assert size(1, 2, 1, 40, 40, 64, w, ctypes.byref(n)) == _lib.H3A_ERR_UNSUPPORTED
     assert n.value == 7
-    assert size(1, 2, 1, 1025, 1300, 128, w, ctypes.byref(n)) == 0 and n.value == 0  # more than 1024 rows: no split
+    assert size(1, 2, 1, 8193, 8193, 128, w, ctypes.byref(n)) == 0 and n.value == 0  # more than 8192 rows: no split
 
 
 def test_backward_refusals():
