@@ -2,9 +2,9 @@
 
 Python side of libh3attn: tensor entry points (ops), the block-sparse h3_sla
 path (sla), windowed attention forward and backward (window), the
-layer norm and prologue around it, forward and backward (block), the ComfyUI
-drop-in hooks (hooks), RoPE tables (rope), HIP-graph capture of layer sequences
-(graphs) and per-component timing (profiling).  All arithmetic happens in the
+layer norm and prologue around it, forward and backward (block), differentiable
+forms of these (autograd), the ComfyUI drop-in hooks (hooks), RoPE tables (rope),
+HIP-graph capture of layer sequences (graphs) and per-component timing (profiling).  All arithmetic happens in the
 HIP kernels of libh3attn.so; nothing here computes attention on the CPU.
 """
 from ._lib import H3AError, LIB_PATH, version
@@ -17,5 +17,6 @@ from .window import attn_bwd_window, attn_fwd_window
 __all__ = [
     "H3AError", "LIB_PATH", "version", "attn_fwd", "attn_fwd_blocksparse", "block_map_to_lut",
     "attn_bwd_window", "attn_fwd_window", "kernel_attrs", "layer_norm_bwd", "layer_norm_fwd",
-    "qk_rmsnorm_rope_", "qk_rmsnorm_rope_axes", "qk_rmsnorm_rope_axes_bwd", "rms_rope_split_half_", "test_qk", "test_pv", "rope_freqs",
+    "qk_rmsnorm_rope_", "qk_rmsnorm_rope_axes", "qk_rmsnorm_rope_axes_bwd", "rms_rope_split_half_",
+    "test_qk", "test_pv", "rope_freqs",
 ]
