@@ -370,7 +370,12 @@ __device__ __forceinline__ void each_seen_key(const WindowArgs &a, const Span &s
 
 // Forward.  A workgroup takes 128 query rows of one head, a wave 32 of them; the
 // 64-key stages of their window are double-buffered in LDS by DMA, two workgroups to a
-// CU, so that one's softmax overlaps the other's MFMAs.
+// CU, so that one's softmax overlaps the other's MFMAs.  The softmax runs against a stale
+// maximum (a row's maximum per stage instead: 9.27 ms for 9.10 at H=56 S=42120 with 4096
+// keys to either side and 512 first ones, 780 us for 763 at B=2 H=56 S=8192, 1024 and
+// 256).  Bound by the MFMAs: 1.09 PFLOP/s of the visible pairs there, a large library
+// matrix product reaching 1.21.  Two groups of four waves that take turns at the MFMAs
+// and the softmax, a barrier after each turn: 1.21 ms for 0.73 at S=8192.
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_fwd_kernel(WindowArgs a) {
   using L = SwzLayout;
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][StageBytes<L>::kK / 2], vbuf[2][StageBytes<L>::kV / 2];
@@ -420,7 +425,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         stage_single<L, ValueLayout>(kbuf[P], vbuf[P], qf, k_rd, v_rd, o,
                                      [&](f32x16(&s)[2], u32x4(&pf)[4]) __attribute__((always_inline)) {
                                        if (c == kPart) mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, kNegInf);
-                                       softmax_stage<2>(s, 0, kBN, g, a.sl2, m, lsum, o, pf);
+                                       softmax_stage_stale<2, true>(s, 0, kBN, g, a.sl2, m, lsum, o, pf);
                                      });
       wait_vmem_all();
       __syncthreads();
