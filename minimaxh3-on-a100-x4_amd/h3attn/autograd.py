@@ -12,8 +12,8 @@ from __future__ import annotations
 
 import torch
 
-from .block import layer_norm_bwd, layer_norm_fwd, qk_rmsnorm_rope_axes, qk_rmsnorm_rope_axes_bwd
-from .window import attn_bwd_window, attn_fwd_window
+from .block import layer_norm_bwd, layer_norm_fwd, qk_rmsnorm_rope_axes, qk_rmsnorm_rope_axes_bwd, whole_numbers
+from .window import attn_bwd_window, attn_fwd_window, mask_args
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -40,6 +40,8 @@ class _WindowAttention(torch.autograd.Function):
 def window_attention(q, k, v, window, sinks: int = 0, causal: bool = False, scale: float | None = None,
                      q_start=None, kv_lens=None) -> torch.Tensor:
     """attn_fwd_window with gradients for q, k and v."""
+    window, sinks = mask_args(window, sinks)
+    scale = None if scale is None else float(scale)
     kw = dict(window=window, sinks=sinks, causal=causal, scale=scale, q_start=q_start, kv_lens=kv_lens)
     return _WindowAttention.apply(q, k, v, kw)
 
@@ -48,7 +50,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, qw, kw, axes, eps, theta):
         ctx.save_for_backward(q, k, pos, qw, kw)
-        ctx.args = (tuple(axes), eps, theta)
+        ctx.args = (axes, eps, theta)
         return qk_rmsnorm_rope_axes(q, k, pos, axes, qw, kw, eps=eps, theta=theta)
 
     @staticmethod
@@ -65,7 +67,7 @@ class _QkNormRope(torch.autograd.Function):
 
 def qk_norm_rope(q, k, pos, axes, qw, kw, eps: float = 1e-6, theta: float = 10000.0):
     """qk_rmsnorm_rope_axes (out of place) with gradients for q, k and the weights, those in the weights' dtype."""
-    return _QkNormRope.apply(q, k, pos, qw, kw, axes, eps, theta)
+    return _QkNormRope.apply(q, k, pos, qw, kw, whole_numbers("axes", axes), float(eps), float(theta))
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -96,4 +98,5 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-6, segments=None, modulate: bool = False) -> torch.Tensor:
     """layer_norm_fwd with gradients for x, weight and bias, each in its own dtype."""
-    return _LayerNorm.apply(x, weight, bias, eps, None if segments is None else tuple(segments), modulate)
+    segments = None if segments is None else whole_numbers("segments", segments)
+    return _LayerNorm.apply(x, weight, bias, float(eps), segments, bool(modulate))

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 
 import torch
 
@@ -14,6 +15,14 @@ from ._lib import check, lib, strides3
 from .ops import HEAD_DIM, _layout, _on_device, _stream
 
 DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
+
+
+def whole_numbers(name: str, values) -> tuple:
+    """values as plain ints: read now, whatever may be written to them later."""
+    try:
+        return tuple(map(operator.index, values))
+    except TypeError:
+        raise ValueError(f"{name} must be whole numbers, got {values!r}") from None
 
 
 # ---------------------------------------------------------------------------
@@ -55,13 +64,13 @@ def _axes_dims(axes: tuple):
     """Checked rotated dims of each axis as the entry points take them."""
     if not 1 <= len(axes) <= _lib.MAX_AXES:
         raise ValueError(f"axes must name the rotated dims of 1 to {_lib.MAX_AXES} axes, got {axes}")
-    if any(d != int(d) or d <= 0 or d % 2 for d in axes) or sum(axes) > HEAD_DIM or sum(axes) % 16:
+    if any(d <= 0 or d % 2 for d in axes) or sum(axes) > HEAD_DIM or sum(axes) % 16:
         raise ValueError(f"axes {axes}: even dims that add up to a multiple of 16, at most {HEAD_DIM}")
-    return (ctypes.c_int * _lib.MAX_AXES)(*(int(d) for d in axes))
+    return (ctypes.c_int * _lib.MAX_AXES)(*axes)
 
 
 def _positions(pos: torch.Tensor, axes, theta, B: int, S: int, device):
-    axes = tuple(axes)
+    axes = whole_numbers("axes", axes)
     dims, A, shape = _axes_dims(axes), len(axes), pos.shape
     if pos.dtype not in (torch.int32, torch.float32) or pos.device != device:
         raise ValueError(f"positions must be int32 or float32 on q's device, got {pos.dtype} on {pos.device}")
@@ -153,7 +162,7 @@ def _bounds(segments, rows: int, groups):
         raise ValueError(f"segments must be non-decreasing bounds from 0 to {rows} rows, got {segments}")
     if groups is not None and groups != len(segments) - 1:
         raise ValueError(f"{len(segments) - 1} segments, but weights for {groups}")
-    return (ctypes.c_int * len(segments))(*(int(b) for b in segments))
+    return (ctypes.c_int * len(segments))(*segments)
 
 
 def _norm_rows(name: str, t: torch.Tensor, C: int) -> torch.Tensor:
@@ -186,7 +195,7 @@ def _norm_prepare(x, weight, bias, segments):
         if groups is not None and n != groups:
             raise ValueError("weight and bias must have the same segments")
         groups = n
-    bounds = _bounds(None if segments is None else tuple(segments), rows, groups)
+    bounds = _bounds(None if segments is None else whole_numbers("segments", segments), rows, groups)
     dt = DTYPES[affine[0][1].dtype] if affine else _lib.FP32
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     return rows, C, bounds, dt, weight, bias

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 
 import torch
 
@@ -22,13 +23,35 @@ from .ops import HEAD_DIM, _as_kernel_input, _layout, _on_device, _stream
 SPLIT_ROWS = 8192
 
 
+def _whole(name: str, n) -> int:
+    """n as a plain int: read now, whatever may be written to it later."""
+    try:
+        return operator.index(n)
+    except TypeError:
+        raise ValueError(f"{name} must be a whole number, got {n!r}") from None
+
+
 def _side(name: str, n) -> int:
-    """A window side as an int; None is no limit."""
+    """A window side; None is no limit."""
     if n is None:
         return 2 ** 31 - 1
-    if int(n) != n or n < 0:
+    if n < 0:
         raise ValueError(f"{name} must be a whole number >= 0 (or None for no limit), got {n}")
-    return min(int(n), 2 ** 31 - 1)
+    return min(n, 2 ** 31 - 1)
+
+
+def mask_args(window, sinks):
+    """The window and the number of first keys as plain ints (None: no limit)."""
+    if not isinstance(window, (tuple, list)) or len(window) != 2:
+        raise ValueError(f"window must be a pair (left, right), got {window!r}")
+    left, right = window
+    if type(left) is not int and left is not None:
+        left = _whole("window's left side", left)
+    if type(right) is not int and right is not None:
+        right = _whole("window's right side", right)
+    if type(sinks) is not int and sinks is not None:
+        sinks = _whole("sinks", sinks)
+    return (left, right), sinks
 
 
 def _per_sequence(name: str, t: torch.Tensor, B: int, device) -> int:
@@ -40,9 +63,7 @@ def _per_sequence(name: str, t: torch.Tensor, B: int, device) -> int:
 
 @functools.lru_cache(maxsize=1024)
 def _sides(window, sinks, causal, start, Sq, Skv):
-    """(left, right, sinks, causal, start) of a checked window; start None: given per sequence."""
-    if not isinstance(window, tuple) or len(window) != 2:
-        raise ValueError(f"window must be a pair (left, right), got {window!r}")
+    """(left, right, sinks, causal, start) of a checked window, all from plain values; start None: given per sequence."""
     left, right = _side("window's left side", window[0]), _side("window's right side", window[1])
     if causal and window[1] not in (0, None):
         raise ValueError(f"a causal window has no right side, got {window[1]}")
@@ -53,14 +74,13 @@ def _sides(window, sinks, causal, start, Sq, Skv):
 
 def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device):
     """The call's h3a_window, and what its workspace's size depends on."""
-    if isinstance(window, list):
-        window = tuple(window)
+    window, sinks = mask_args(window, sinks)
     lens = None if kv_lens is None else _per_sequence("kv_lens", kv_lens, B, device)
     starts = None
     if isinstance(q_start, torch.Tensor):
         starts, start = _per_sequence("q_start", q_start, B, device), None
     elif q_start is not None:
-        start = int(q_start)
+        start = _whole("q_start", q_start)
     elif lens is not None and Sq != Skv:
         raise ValueError("kv_lens with Sq != Skv needs q_start: where the queries sit in the sequences")
     else:

@@ -114,3 +114,39 @@ def test_python_refusals(monkeypatch):
         h3attn.attn_bwd_window(q.float(), q, q, q, q, lse, (1, 1))
     with pytest.raises(ValueError, match="lse"):
         h3attn.attn_bwd_window(q, q, q, q, q, lse[:, :, :7], (1, 1))
+
+
+class Count:
+    """A whole number that can be written to, as a 0-d tensor can."""
+
+    def __init__(self, n):
+        self.n = n
+
+    def __index__(self):
+        return self.n
+
+
+def test_arguments_are_read_at_each_call():
+    from h3attn import autograd, block, window
+    cpu, n = torch.device("cpu"), Count(2)
+    read = lambda: window._window([n, n], n, False, n, None, 1, 4, 16, cpu)[1]  # noqa: E731
+    assert read() == (2, 2, 2, 0, 2)
+    n.n = 3
+    assert read() == (3, 3, 3, 0, 3)
+    t = torch.tensor(5)
+    assert window.mask_args((t, None), t) == ((5, None), 5)
+    t += 1
+    assert window.mask_args((t, None), t) == ((6, None), 6)
+    pos = torch.zeros(4, 1, dtype=torch.int32)
+    n.n = 32
+    assert block._positions(pos, [n], 1e4, 1, 4, cpu)[1].dims[0] == 32
+    n.n = 64
+    assert block._positions(pos, [n], 1e4, 1, 4, cpu)[1].dims[0] == 64
+    assert block.whole_numbers("segments", torch.tensor([0, 4, 9])) == (0, 4, 9)
+    for bad in ([0, 1.5], [0, None], ["0"]):
+        with pytest.raises(ValueError, match="segments must be whole numbers"):
+            block.whole_numbers("segments", bad)
+    q = torch.zeros(1, 1, 4, 128, dtype=torch.bfloat16)
+    for kw in ({"window": (1, 0.5)}, {"window": (1, 1), "sinks": 2.0}, {"window": 4}):
+        with pytest.raises(ValueError, match="window|sinks"):
+            autograd.window_attention(q, q, q, **kw)
