@@ -247,7 +247,7 @@ typedef struct {
  * Forward.  lse [B,H,Sq] fp32 contiguous (may be NULL): log of the sum of
  * exp(scale * q.k) over the keys seen, for h3a_attn_bwd_window.  Strides and
  * alignment as h3a_attn_fwd, and every sequence stride < 2^24 elements; lengths
- * up to 2^29.  Range: max|v| as for h3a_attn_fwd, with the keys a row sees for Skv.
+ * up to 2^29 and B * H * ceil(longer / 128) up to 2^22.  Range: max|v| as for h3a_attn_fwd, with the keys a row sees for Skv.
  * workspace: h3a_attn_fwd_window_workspace_size bytes for the current
  * device (0, so NULL, for more than 8192 rows: fewer may be split along the keys),
  * untouched until the call's work has completed.  No counterpart in the reference.

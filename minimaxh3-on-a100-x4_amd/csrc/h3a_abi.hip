@@ -146,9 +146,11 @@ int check_window_sizes(int B, int H, int Hkv, int Sq, int Skv, int D) {
   if (D != 128) return fail(H3A_ERR_UNSUPPORTED, "head_dim %d unsupported (only 128)", D);
   if (H % Hkv != 0) return fail(H3A_ERR_INVALID_ARG, "%d key heads do not divide %d heads", Hkv, H);
   if (Sq > kMaxWindowLen || Skv > kMaxWindowLen) return fail(H3A_ERR_INVALID_ARG, "sequence too long");
-  // Workgroups of the largest launch, one per 128 rows of a head.
+  // The largest launch has three workgroups of 256 threads per 128 rows of a head at most,
+  // and a launch fewer than 2^32 threads.
   const int64_t longest = Sq > Skv ? Sq : Skv;
-  if ((int64_t)B * H * ((longest + 127) / 128) > INT_MAX) return fail(H3A_ERR_UNSUPPORTED, "too many query or key tiles");
+  if ((int64_t)B * H * ((longest + 127) / 128) > 1 << 22)
+    return fail(H3A_ERR_UNSUPPORTED, "more than 2^22 tiles of 128 rows (B=%d H=%d, %lld rows)", B, H, (long long)longest);
   return H3A_OK;
 }
 

@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 //
 // The first keys are seen by every query, the others by a window's: tiles that hold
 // first keys are cut into a.pieces equal runs of stages, which leave fp32 partial sums
-// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being the shortest.
+// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being short.
 constexpr int kQStage = 64;
 struct DkdvLds {
   uint16_t q[2][kQStage * 128], dout[2][kQStage * 128];
@@ -1029,12 +1029,18 @@ __global__ void __launch_bounds__(256) window_dkdv_sum_kernel(WindowArgs a) {
 }
 
 // Tiles that hold first keys, and the runs each is cut into: as many as make a run no
-// longer than a window tile's.
+// longer than a window tile's, or than a quarter of what one of the chip's 512 places for
+// workgroups has to do in all, if that is more (it also bounds the partial sums: at most
+// about 1024 runs of 128 KB).  In stages of one query head.
 static void plan_dkdv(WindowArgs &a) {
-  const int64_t range = (int64_t)kRows + a.left + a.right;
   a.nkt = (a.Skv + kRows - 1) / kRows;
   a.first_tiles = (a.sinks + kRows - 1) / kRows;
-  a.pieces = (int)((a.Sq + range - 1) / range);
+  const int64_t all_rows = (a.Sq + kQStage - 1) / kQStage, heads = (int64_t)a.B * a.Hkv;
+  int64_t run = ((int64_t)kRows + a.left + a.right + kQStage - 1) / kQStage;
+  if (run > all_rows) run = all_rows;
+  const int64_t share = 2 * heads * (a.first_tiles * all_rows + (a.nkt - a.first_tiles) * run) / (4 * 512);
+  if (run < share) run = share;
+  a.pieces = (int)((all_rows + run - 1) / run);
   if (a.first_tiles == 0 || a.pieces == 1) {
     a.first_tiles = 0;
     a.pieces = 1;
@@ -1055,10 +1061,13 @@ size_t window_bwd_bytes(WindowArgs a) {
 constexpr int kRowRuns = 256, kKeyRuns = 128;
 // Grid of `tiles` work items for each of `heads` heads (item_of), in `runs` runs or more.
 static int deal(int tiles, int heads, int runs_wanted, int *chunk) {
+  *chunk = 1;
+  if (tiles == 0) return 0;
   const int64_t total = (int64_t)heads * tiles, most = total / runs_wanted;
-  *chunk = most < 1 ? 1 : (most > 64 ? 64 : (int)most);
-  const int64_t runs = (int64_t)heads * ((tiles + *chunk - 1) / *chunk);
-  return (int)((runs + 7) / 8 * 8 * *chunk);
+  const int longest = most < 1 ? 1 : (most > 64 ? 64 : (int)most);
+  const int per_head = (tiles + longest - 1) / longest;
+  *chunk = (tiles + per_head - 1) / per_head;  // a head's runs alike
+  return (int)(((int64_t)heads * per_head + 7) / 8 * 8 * *chunk);
 }
 
 // Query rows up to which splitting the keys is weighed against the tiles.

@@ -65,6 +65,17 @@ def test_sinks(gpu, sinks, causal):
     check(gpu, 1, 1, 1, 700, 700, (50, 0 if causal else 20), sinks, causal, seed=sinks)
 
 
+def test_first_keys_of_many_heads(gpu):
+    # Runs of queries longer than a window tile's: 4 of 7 stages each, 24 stages in all.
+    check(gpu, 1, 28, 28, 1500, 1500, (0, 0), 2 ** 31 - 1, False, seed=5)
+
+
+@pytest.mark.parametrize("B,H,S", [(40, 6, 3), (300, 2, 1), (9, 14, 128)])
+def test_many_short_sequences(gpu, B, H, S):
+    # More heads than runs of tiles: every head's tiles are dealt, and none twice.
+    check(gpu, B, H, H // 2, S, S, (2, 1), 1, False, seed=B)
+
+
 @pytest.mark.parametrize("window", [(0, 0), (1, 0), (63, 64), (64, 63), (200, 0), (0, 200), (511, 511), (2000, 2000)])
 def test_window_sides(gpu, window):
     check(gpu, 1, 2, 1, 513, 513, window, 3, False, seed=window[0])

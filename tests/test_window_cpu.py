@@ -150,3 +150,29 @@ def test_arguments_are_read_at_each_call():
     for kw in ({"window": (1, 0.5)}, {"window": (1, 1), "sinks": 2.0}, {"window": 4}):
         with pytest.raises(ValueError, match="window|sinks"):
             autograd.window_attention(q, q, q, **kw)
+
+
+def test_backward_workspace_is_bounded():
+    """First keys are cut into runs of queries that leave partial sums: a bounded number of them."""
+    L = _lib.lib()
+    n = ctypes.c_size_t(0)
+
+    def size(B, H, Hkv, S, left, right, sinks):
+        w = _lib.Window(left, right, sinks, 0, 0, None, None)
+        assert L.h3a_attn_bwd_window_workspace_size(B, H, Hkv, S, S, 128, ctypes.byref(w), ctypes.byref(n)) == 0
+        return n.value - 2 * 4 * B * H * S  # beside the rows' statistics
+
+    run = 2 * 128 * 128 * 4
+    for args in ((1, 56, 56, 42120, 0, 0, 42120), (1, 56, 8, 42120, 64, 64, 4096), (1, 1, 1, 1 << 22, 0, 0, 1 << 20),
+                 (2, 56, 8, 8192, 16, 16, 256), (16, 56, 56, 8192, 0, 0, 2 ** 31 - 1), (1, 1, 1, 1 << 29, 0, 0, 1 << 29)):
+        B, H, Hkv, S, left, right, sinks = args
+        tiles = B * Hkv * ((min(sinks, S) + 127) // 128)
+        assert 0 <= size(*args) <= (1024 + min(tiles, 1024)) * run + 512, args
+
+
+def test_tiles_past_a_launch_are_refused():
+    L = _lib.lib()
+    assert _fwd(L, B=1 << 11, H=1 << 11, Hkv=1 << 11, w=None) == _lib.H3A_ERR_INVALID_ARG  # 2^22: sizes pass
+    assert _fwd(L, B=(1 << 11) + 1, H=1 << 11, Hkv=1 << 11) == _lib.H3A_ERR_UNSUPPORTED
+    assert _fwd(L, B=1 << 20, H=4, Hkv=4, Sq=129, Skv=129) == _lib.H3A_ERR_UNSUPPORTED
+    assert b"tiles" in L.h3a_last_error()
