@@ -443,7 +443,7 @@ int h3a_qk_rmsnorm_rope_axes_bwd(const void *q_dout, const void *k_dout, const v
  * bounds is host memory, segments + 1 non-decreasing ints from 0 to rows; a segment
  * may be empty.  x and y share dtype; w and b share w_dtype (H3A_BF16, H3A_FP16 or
  * H3A_FP32).  mean, rstd [rows] fp32 (both or neither NULL) are kept for the
- * backward.  y may be x.  rows may be 0; C <= 16384.
+ * backward.  y may be x.  rows from 0 to 2^30; C <= 16384.
  */
 #define H3A_BF16 0
 #define H3A_FP16 1

@@ -260,6 +260,7 @@ size_t rope_axes_bwd_bytes(int B, int S) { return (size_t)rope_axes_bwd_wgs(B, S
 int check_norm(int rows, int C, int dtype, int w_dtype, const int *bounds, int segments) {
   if (rows < 0 || C <= 0) return fail(H3A_ERR_INVALID_ARG, "bad sizes (rows=%d C=%d)", rows, C);
   if (C > 16384) return fail(H3A_ERR_UNSUPPORTED, "%d channels unsupported (at most 16384)", C);
+  if (rows > 1 << 30) return fail(H3A_ERR_UNSUPPORTED, "%d rows unsupported (at most 2^30)", rows);
   for (int d : {dtype, w_dtype})
     if (d != H3A_BF16 && d != H3A_FP16 && d != H3A_FP32) return fail(H3A_ERR_UNSUPPORTED, "dtype %d unsupported", d);
   if (!bounds || segments <= 0) return fail(H3A_ERR_INVALID_ARG, "no segments");

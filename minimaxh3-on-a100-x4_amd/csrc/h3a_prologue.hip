@@ -514,6 +514,8 @@ __global__ void __launch_bounds__(256) rope_axes_param_grad_kernel(RopeAxesArgs 
   if (threadIdx.x < 4) a.dw[at >> 7][at & 127] = (fold[0][col] + fold[1][col]) + (fold[2][col] + fold[3][col]);
 }
 
+// Forward: workgroups at most (a launch has fewer than 2^32 threads; the kernel walks on).
+constexpr int64_t kAxesMaxWgs = 1 << 22;
 // Backward: workgroups that each leave a partial row of the weights' gradients.
 int rope_axes_bwd_wgs(int B, int S) {
   const int64_t n = ((int64_t)B * S + kAxesTokens - 1) / kAxesTokens;
@@ -523,7 +525,7 @@ int rope_axes_bwd_wgs(int B, int S) {
 template <bool kBwd>
 static int launch_rope_axes_as(const RopeAxesArgs &a, hipStream_t s) {
   const int64_t groups = ((int64_t)a.B * a.S + kAxesTokens - 1) / kAxesTokens;
-  const int64_t wgs = kBwd ? rope_axes_bwd_wgs(a.B, a.S) : groups;
+  const int64_t wgs = kBwd ? rope_axes_bwd_wgs(a.B, a.S) : (groups < kAxesMaxWgs ? groups : kAxesMaxWgs);
   const bool full = a.rot == kRopeD;
   const int h = a.H[0] > a.H[1] ? a.H[0] : a.H[1];
   void (*kernel)(RopeAxesArgs) =

@@ -150,8 +150,8 @@ def qk_rmsnorm_rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor
 @functools.lru_cache(maxsize=256)
 def _bounds(segments, rows: int, groups):
     """Checked bounds of the segments as the entry points take them; None: `groups` equal ones."""
-    if rows > 2 ** 31 - 1:
-        raise ValueError("too many rows")
+    if rows > 2 ** 30:
+        raise ValueError(f"{rows} rows unsupported (at most 2^30)")
     if segments is None:
         groups = groups or 1
         if rows % groups:

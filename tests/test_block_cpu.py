@@ -127,3 +127,14 @@ def test_references_against_differences():
             down = fn()
             flat[i] = v
             assert abs((up - down) / (2 * h) - gflat[i].item()) < 1e-6 * (1 + abs(gflat[i].item()))
+
+
+def test_norm_rows_past_the_limit():
+    L = _lib.lib()
+    rows = (1 << 30) + 1
+    bounds = (ctypes.c_int * 2)(0, rows)
+    assert L.h3a_layer_norm_fwd(16, 64, 16, 16, 16, 64, None, None, rows, 64, 0, 2, bounds, 1, 0, 1e-6,
+                                None) == _lib.H3A_ERR_UNSUPPORTED
+    assert L.h3a_layer_norm_bwd_workspace_size(bounds, 1, 64, ctypes.byref(ctypes.c_size_t(0))) == _lib.H3A_ERR_UNSUPPORTED
+    with pytest.raises(ValueError, match="rows"):
+        block._bounds(None, rows, None)

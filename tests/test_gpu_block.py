@@ -173,6 +173,18 @@ def test_rope_lengths(gpu, B, S):
         check_rope(*(c := rope_case(gpu, B, S, 3, 2, axes, S, dtype, batched))[:3], axes, *c[3:])
 
 
+def test_rope_more_tokens_than_a_launch_walks_at_once(gpu):
+    # 2^24 tokens are taken by 2^22 workgroups in one step; offsets pass 32 bits on the way.
+    S = (1 << 24) + 7
+    q, k = (torch.randn(1, S, 1, 128, device=gpu, dtype=torch.bfloat16) for _ in range(2))
+    pos = (torch.arange(S, device=gpu, dtype=torch.int32) % 4099)[:, None].contiguous()
+    w = torch.rand(128, device=gpu).to(torch.bfloat16) + 0.5
+    oq, ok = h3attn.qk_rmsnorm_rope_axes(q, k, pos, (128,), w, w)
+    for a, b in ((0, 9), (S // 2, S // 2 + 9), ((1 << 24) - 5, (1 << 24) + 3), (S - 7, S)):
+        for whole, part in zip((oq, ok), h3attn.qk_rmsnorm_rope_axes(q[:, a:b], k[:, a:b], pos[a:b], (128,), w, w)):
+            assert torch.equal(whole[:, a:b], part)
+
+
 def test_rope_far_positions(gpu):
     """Positions up to 2^30: the angles stay those of the definition."""
     axes = (44, 42, 42)
