@@ -157,15 +157,21 @@ __device__ __forceinline__ void two_buffers(int n, Stage stage) {
 }
 
 // A wave's 32 rows as columns of an MFMA operand, straight from global memory; rows
-// past `rows` are zeros.
-__device__ __forceinline__ void load_columns(u32x4 (&f)[8], const uint16_t *base, int64_t stride, int row, int rows,
-                                             int g) {
+// past `rows` are zeros: the loads (row 0 for those), and what makes them zeros.
+__device__ __forceinline__ void issue_columns(u32x4 (&f)[8], const uint16_t *base, int64_t stride, int row, int rows,
+                                              int g) {
   const uint16_t *p = base + (int64_t)(row < rows ? row : 0) * stride + 8 * g;
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) {
-    const u32x4 v = *(const u32x4 *)(p + 16 * ks);
-    f[ks] = row < rows ? v : u32x4{0, 0, 0, 0};
-  }
+  for (int ks = 0; ks < 8; ++ks) f[ks] = *(const u32x4 *)(p + 16 * ks);
+}
+__device__ __forceinline__ void clear_past(u32x4 (&f)[8], int row, int rows) {
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) f[ks] = row < rows ? f[ks] : u32x4{0, 0, 0, 0};
+}
+__device__ __forceinline__ void load_columns(u32x4 (&f)[8], const uint16_t *base, int64_t stride, int row, int rows,
+                                             int g) {
+  issue_columns(f, base, stride, row, rows, g);
+  clear_past(f, row, rows);
 }
 
 // acc * mul, rounded to bf16, to rows row0 .. row0 + nrows - 1: through a wave-private
@@ -672,9 +678,25 @@ __global__ void __launch_bounds__(256) window_token_sum_kernel(WindowArgs a, int
   if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Sq + row] = log_sum(top, l);
 }
 
+// Whether a run of positions p0 .. p1 holds one that sees no more than a stage of keys (the
+// window's part of the count is least at an end of the run).
+__device__ __forceinline__ bool few_keys(const WindowArgs &a, const Span &s, int p0, int p1) {
+  KeyStages<1> st0, st1;
+  st0.init(a, s, p0, p0);
+  st1.init(a, s, p1, p1);
+  return st0.n <= kBN || st1.n <= kBN;
+}
+
 // Backward, dQ: tiles and stages as forward, with P from the stored lse.  The rows' lse
 // (log2 units; +inf, so that p = 0, for a row that saw nothing) and delta = dO.O go to
-// a.stats for the second kernel.
+// a.stats for the second kernel.  O's rounding to bf16 makes delta off by 2^-9 of what the
+// few keys of a row near a sequence's start or under a narrow window give, which there is
+// as much as dS itself (a row of one key has dS = 0): such tiles take sum p dP in a pass of
+// their own instead (relative error of dQ and dK, S=100 causal: 0.0029 -> 0.0024, which is
+// the rounding of dS and of the result; from 64 keys on delta's part is under a fifth).
+// The pass takes 55 us of a backward's 319 at H=56/8 S=8192 with 17 keys to a row.
+// Bound by the MFMAs: 0.99 ms for the 1.06 TFLOP of B=2 H=56/8 S=8192, 1024 keys to either
+// side and 256 first ones, one sequence less than half as long.
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dq_kernel(WindowArgs a) {
   using L = DualLayout;
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][StageBytes<L>::kK / 2], vbuf[2][StageBytes<L>::kK / 2];
@@ -709,26 +731,53 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       fetch_tile(vdma, Vb, a.vss, st.key0(j), st.limit(j), vbuf[P]);
     };
     fetch(0, C<0>{});
-    u32x4 qf[8], df[8];
-    load_columns(qf, a.q + it.b * a.qsb + it.h * a.qsh, a.qss, row, a.Sq, g);
-    load_columns(df, a.dout + it.b * a.gsb + it.h * a.gsh, a.gss, row, a.Sq, g);
-    {
-      u32x4 of[8];
-      load_columns(of, a.o + it.b * a.osb + it.h * a.osh, a.oss, row, a.Sq, g);
+    // All of them in flight at once.
+    u32x4 qf[8], df[8], of[8];
+    const int64_t stat = ((int64_t)it.b * a.H + it.h) * a.Sq + (row < a.Sq ? row : a.Sq - 1);
+    issue_columns(qf, a.q + it.b * a.qsb + it.h * a.qsh, a.qss, row, a.Sq, g);
+    issue_columns(df, a.dout + it.b * a.gsb + it.h * a.gsh, a.gss, row, a.Sq, g);
+    issue_columns(of, a.o + it.b * a.osb + it.h * a.osh, a.oss, row, a.Sq, g);
+    const float lse = a.lse[stat];
+    pin_order();
+    clear_past(qf, row, a.Sq);
+    clear_past(df, row, a.Sq);
+    clear_past(of, row, a.Sq);
+    l2 = lse == kNegInf ? -kNegInf : lse * kLog2e;
+    const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
+    if (few_keys(a, sp, sp.qs + r0, sp.qs + r1)) {
+      wait_vmem_all();
+      __syncthreads();
+      two_buffers(st.n, [&](auto par, int j) __attribute__((always_inline)) {
+        constexpr int P = decltype(par)::value;
+        if (j + 1 < st.n) fetch(j + 1, C<P ^ 1>{});
+        f32x16 s[2], dp[2];
+        score_tile<L, 2>(kbuf[P], qf, k_rd, s);
+        score_tile<L, 2>(vbuf[P], df, k_rd, dp);
+        const int key0 = st.key0(j) + 4 * g, low = j < st.n_first ? 1 << 30 : lo;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = key0 + 32 * u + 8 * (r >> 2) + (r & 3);
+            if ((at >= low && at <= hi) || at < first)
+              delta = fmaf(fast_exp2(fmaf(s[u][r], a.sl2, -l2)), dp[u][r], delta);
+          }
+        wait_vmem_all();
+        __syncthreads();
+      });
+      if (st.n > 2) fetch(0, C<0>{});  // (two stages are both still there)
+    } else {
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           delta = fmaf(bf16_hi(of[ks][i]), bf16_hi(df[ks][i]), fmaf(bf16_lo(of[ks][i]), bf16_lo(df[ks][i]), delta));
-      delta = half_swap_sum(delta);
     }
-    const int64_t stat = ((int64_t)it.b * a.H + it.h) * a.Sq + (row < a.Sq ? row : a.Sq - 1);
-    l2 = a.lse[stat] == kNegInf ? -kNegInf : a.lse[stat] * kLog2e;
+    delta = half_swap_sum(delta);
     if (g == 0 && row < a.Sq) {
       a.stats[stat] = l2;
       a.stats[a.stats_n + stat] = delta;
     }
-    const int k_rd = L::k_base(l32, g), t_rd = L::v_base(lane);
     wait_vmem_all();
     __syncthreads();
     two_buffers(st.n, [&](auto par, int j) __attribute__((always_inline)) {
@@ -784,7 +833,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // waves per SIMD wait for every operand and spill: 2.7 ms at B=2 H=56/8 S=8192 with 1024
 // keys to either side); alone on its SIMD it moves scores between register files for as
 // long as it multiplies (3.5 ms); and waves of both kinds in one workgroup run their
-// softmax at the same time (2.9 ms).
+// softmax at the same time (2.9 ms).  As it is: 1.95 ms there, 0.91 PFLOP/s of the five
+// products, the rest being the tail of the grid (seven heads share a tile's keys, so an
+// item is 238 stages and a place gets four or five of them) and the masked stages.
 //
 // The first keys are seen by every query, the others by a window's: tiles that hold
 // first keys are cut into a.pieces equal runs of stages, which leave fp32 partial sums

@@ -65,6 +65,23 @@ def test_sinks(gpu, sinks, causal):
     check(gpu, 1, 1, 1, 700, 700, (50, 0 if causal else 20), sinks, causal, seed=sinks)
 
 
+@pytest.mark.parametrize("S", [1, 40, 300])
+def test_rows_of_one_key_have_no_score_gradient(gpu, S):
+    # P = 1, so dS = P (dP - P dP) = 0.  In fp32: s and lse agree to 2^-19 (|lse| < 8 in three
+    # roundings, an exp2 and a log2 of an ulp), so |1 - P| < 2^-18 and |dS| < 2^-18 |dP|; the
+    # roundings of dS and of the result add a 2^-7th of that.
+    q, k, v, do = make(gpu, 1, 2, 2, S, S, seed=S)
+    o, lse = h3attn.attn_fwd_window(q, k, v, (0, 0), return_lse=True)
+    assert lse.abs().max() < 8
+    dq, dk, _ = (t.double() for t in h3attn.attn_bwd_window(do, q, k, v, o, lse, (0, 0)))
+    dp = (do.double() * v.double()).sum(-1, keepdim=True).abs()
+    assert (dq.abs() <= 2.0 ** -17 * SCALE * dp * k.double().abs()).all()
+    assert (dk.abs() <= 2.0 ** -17 * SCALE * dp * q.double().abs()).all()
+    dq, _, _ = h3attn.attn_bwd_window(do, q, k, v, *h3attn.attn_fwd_window(q, k, v, (50, 0), causal=True, return_lse=True),
+                                      (50, 0), causal=True)
+    assert (dq[:, :, 0].double().abs() <= 2.0 ** -17 * SCALE * dp[:, :, 0] * k[:, :, 0].double().abs()).all()
+
+
 def test_first_keys_of_many_heads(gpu):
     # Runs of queries longer than a window tile's: 4 of 7 stages each, 24 stages in all.
     check(gpu, 1, 28, 28, 1500, 1500, (0, 0), 2 ** 31 - 1, False, seed=5)
