@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // waves per SIMD wait for every operand and spill: 2.7 ms at B=2 H=56/8 S=8192 with 1024
 // keys to either side); alone on its SIMD it moves scores between register files for as
 // long as it multiplies (3.5 ms); and waves of both kinds in one workgroup run their
-// softmax at the same time (2.9 ms).  As it is: 1.95 ms there, 0.91 PFLOP/s of the five
+// softmax at the same time (2.9 ms).  As it is: 1.8 to 2.0 ms there, 0.9 PFLOP/s of the five
 // products, the rest being the tail of the grid (seven heads share a tile's keys, so an
 // item is 238 stages and a place gets four or five of them) and the masked stages.
 //
@@ -1106,19 +1106,22 @@ size_t window_bwd_bytes(WindowArgs a) {
   return 2 * stat_rows(a) * sizeof(float) + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
 }
 
-// Runs the tiles are dealt in at least: fewer, longer ones share more of their keys in an
-// XCD's L2 (H=56 S=42120, 4096 keys to either side, forward: 10.0 ms in runs of 16 tiles,
-// 9.2 in runs of 64), more of them level the XCDs' work.
-constexpr int kRowRuns = 256, kKeyRuns = 128;
-// Grid of `tiles` work items for each of `heads` heads (item_of), in `runs` runs or more.
-static int deal(int tiles, int heads, int runs_wanted, int *chunk) {
+// Grid of `tiles` work items for each of a batch's `heads` heads (item_of).  Runs are as long
+// as they can be, up to 64 tiles, with a multiple of 8 to a sequence: neighbours share more of
+// what they read in an XCD's L2, and every XCD gets as many (dK and dV, against runs of a
+// 128th of all tiles: 2.29 -> 2.01 ms at B=2 H=56/8 S=8192, 122 -> 111 us at H=14 S=4104;
+// forward, runs of 16 tiles against 64: 10.0 -> 9.2 ms at H=56 S=42120).  Where sequences may
+// end early, runs that are a part of a head may be empty, so there are at least `ragged_runs`.
+static int deal(const WindowArgs &a, int tiles, int heads, int ragged_runs, int *chunk) {
   *chunk = 1;
   if (tiles == 0) return 0;
-  const int64_t total = (int64_t)heads * tiles, most = total / runs_wanted;
-  const int longest = most < 1 ? 1 : (most > 64 ? 64 : (int)most);
-  const int per_head = (tiles + longest - 1) / longest;
+  int per_head = (tiles + 63) / 64;
+  while (per_head < tiles && (int64_t)heads * per_head % 8) ++per_head;
+  if (a.kv_lens && per_head > 1)
+    while (per_head < tiles && ((int64_t)heads * per_head % 8 || (int64_t)a.B * heads * per_head < ragged_runs)) ++per_head;
   *chunk = (tiles + per_head - 1) / per_head;  // a head's runs alike
-  return (int)(((int64_t)heads * per_head + 7) / 8 * 8 * *chunk);
+  const int64_t runs = (int64_t)a.B * heads * ((tiles + *chunk - 1) / *chunk);
+  return (int)((runs + 7) / 8 * 8 * *chunk);
 }
 
 // Query rows up to which splitting the keys is weighed against the tiles.
@@ -1176,7 +1179,7 @@ int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
   if (rc) return rc;
   if (!plan_token(a, cus)) {
     a.nqt = (a.Sq + kRows - 1) / kRows;
-    const int grid = deal(a.nqt, a.B * a.H, kRowRuns, &a.chunk);
+    const int grid = deal(a, a.nqt, a.H, 256, &a.chunk);
     hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
     return check_launch("window_fwd_kernel");
   }
@@ -1193,14 +1196,14 @@ int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {
   a.stats = static_cast<float *>(ws);
   a.stats_n = (int64_t)stat_rows(a);
   a.nqt = (a.Sq + kRows - 1) / kRows;
-  const int grid = deal(a.nqt, a.B * a.H, kRowRuns, &a.chunk);
+  const int grid = deal(a, a.nqt, a.H, 256, &a.chunk);
   hipLaunchKernelGGL(window_dq_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   int rc = check_launch("window_dq_kernel");
   if (rc) return rc;
   plan_dkdv(a);
   a.part = a.stats + 2 * a.stats_n;
-  a.grid_whole = deal(a.nkt - a.first_tiles, a.B * a.Hkv, kKeyRuns, &a.chunk);
-  a.grid_pieces = deal(a.first_tiles * a.pieces, a.B * a.Hkv, kKeyRuns, &a.chunk_pieces);
+  a.grid_whole = deal(a, a.nkt - a.first_tiles, a.Hkv, 128, &a.chunk);
+  a.grid_pieces = deal(a, a.first_tiles * a.pieces, a.Hkv, 128, &a.chunk_pieces);
   hipLaunchKernelGGL(window_dkdv_kernel, dim3((unsigned)(2 * a.grid_whole + 2 * a.grid_pieces)), dim3(256), 0, s, a);
   rc = check_launch("window_dkdv_kernel");
   if (rc || a.first_tiles == 0) return rc;
