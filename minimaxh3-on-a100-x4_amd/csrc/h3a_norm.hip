@@ -327,28 +327,35 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(NormArgs a) {
 }
 
 // Sums of the partial rows of each segment's workgroups: 64 channels of dw or db per
-// workgroup, its four waves taking every fourth row.
-__global__ void __launch_bounds__(256) layer_norm_param_grad_kernel(NormArgs a) {
-  __shared__ float fold[4][64];
+// workgroup, its waves in turn.  Sixteen waves where segments have over 128 partial rows on
+// average (512 rows of 5376 channels: 10.7 us with four, 4.8 with sixteen), four where they
+// have fewer (39: 6.4 and 8.6).
+template <int kSumWaves>
+__global__ void __launch_bounds__(64 * kSumWaves) layer_norm_param_grad_kernel(NormArgs a) {
+  __shared__ float fold[kSumWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + lane, seg = blockIdx.y, which = blockIdx.z;
   const int w0 = a.wg0 + a.first_wg[seg], w1 = a.wg0 + a.first_wg[seg + 1];
   float sum = 0.f;
   if (c < a.C) {
     constexpr int kFlight = 8;  // loads in flight
-    for (int w = w0 + wave; w < w1; w += 4 * kFlight) {
+    for (int w = w0 + wave; w < w1; w += kSumWaves * kFlight) {
       float v[kFlight];
 #pragma unroll
       for (int i = 0; i < kFlight; ++i)
-        v[i] = w + 4 * i < w1 ? a.partial[((int64_t)(w + 4 * i) * 2 + which) * a.C + c] : 0.f;
+        v[i] = w + kSumWaves * i < w1 ? a.partial[((int64_t)(w + kSumWaves * i) * 2 + which) * a.C + c] : 0.f;
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) sum += v[i];
     }
   }
   fold[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && c < a.C)
-    (which ? a.db : a.dw)[(int64_t)(a.seg0 + seg) * a.C + c] = (fold[0][lane] + fold[1][lane]) + (fold[2][lane] + fold[3][lane]);
+  if (wave == 0 && c < a.C) {
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSumWaves; ++w) sum += fold[w][lane];
+    (which ? a.db : a.dw)[(int64_t)(a.seg0 + seg) * a.C + c] = sum;
+  }
 }
 
 typedef void (*NormKernel)(NormArgs);
@@ -394,8 +401,10 @@ int norm_rows_per_wg(int64_t rows, int C, int segments, bool bwd) {
   const int per_cu = bwd ? (C <= 512 || (C > 1024 && C <= 2048) ? 5 : (C <= 1024 ? 3 : 2)) : (C <= 2048 ? 8 : 4);
   const int wgs = 256 * per_cu - (segments < 128 ? segments : 0);
   const int step = C <= 1024 ? 4 : 1;
-  const int64_t n = (rows + wgs - 1) / wgs;
-  return (int)((n < 1 ? 1 : n) + step - 1) / step * step;
+  // Backward, four rows at least: a workgroup leaves as many bytes of partial sums as a row and
+  // a half has to read and write.
+  const int64_t n = (rows + wgs - 1) / wgs, least = bwd ? 4 : 1;
+  return (int)((n < least ? least : n) + step - 1) / step * step;
 }
 
 int norm_wgs(const int *bounds, int segments, int rows_per_wg) {
@@ -423,8 +432,9 @@ int launch_layer_norm(NormArgs a, const int *bounds, int segments, int dtype, bo
       if (rc) return rc;
     }
     if (bwd && a.partial) {
-      hipLaunchKernelGGL(layer_norm_param_grad_kernel, dim3((unsigned)((a.C + 63) / 64), (unsigned)a.segments, 2),
-                         dim3(256), 0, s, a);
+      const bool many = wgs > 128 * a.segments;
+      hipLaunchKernelGGL((many ? layer_norm_param_grad_kernel<16> : layer_norm_param_grad_kernel<4>),
+                         dim3((unsigned)((a.C + 63) / 64), (unsigned)a.segments, 2), dim3(many ? 1024 : 256), 0, s, a);
       const int rc = check_launch("layer_norm_param_grad_kernel");
       if (rc) return rc;
     }
