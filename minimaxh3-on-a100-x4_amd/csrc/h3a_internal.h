@@ -143,9 +143,10 @@ struct WindowArgs {
   int64_t dvsb, dvsh, dvss;
   float *stats;     // [2][stats_n]: lse in log2 units and dO.O of every row [B,H,Sq]
   int64_t stats_n;
-  int grid_whole, grid_pieces, chunk_pieces;  // workgroups of dK (and of dV) for whole key tiles and for pieces
-  int first_tiles, pieces;  // key tiles cut into runs of queries, and the runs of each
-  float *part;              // their partial sums: [B,Hkv,first_tiles,pieces][dK, dV][128][128]
+  int grid_whole, grid_pieces, chunk_pieces;  // workgroups of dK (and of dV) for the window's key tiles and the first keys'
+  int first_tiles, pieces;  // key tiles that hold first keys and are cut into runs of queries, and the runs of each
+  int rest_pieces;          // runs of each other tile (1: not cut)
+  float *part;              // the runs' partial sums, [..][dK, dV][128][128] (part_slot)
 };
 int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s);
 int window_fwd_bytes(WindowArgs a, size_t *bytes);  // workspace on the current device

@@ -839,15 +839,27 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 //
 // The first keys are seen by every query, the others by a window's: tiles that hold
 // first keys are cut into a.pieces equal runs of stages, which leave fp32 partial sums
-// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being short.
+// in a.part for window_dkdv_sum_kernel.  They come last in the grid, being short.  Where
+// few tiles leave most of the chip idle (heads that share keys on a short sequence), the
+// others are cut too, into a.rest_pieces.
 constexpr int kQStage = 64;
 struct DkdvLds {
   uint16_t q[2][kQStage * 128], dout[2][kQStage * 128];
   float stats[2][2][kQStage];  // lse (log2 units), delta
 };
 
+// Where a piece's dK (which 0) or dV of 128 keys by 128 dims is in a.part: those of the first
+// keys' tiles, then the others'.
+__device__ __forceinline__ int64_t part_slot(const WindowArgs &a, int bh, int tile, int piece, int which) {
+  const int64_t heads = (int64_t)a.B * a.Hkv, rest = a.nkt - a.first_tiles;
+  const int64_t at = tile < a.first_tiles
+                         ? ((int64_t)bh * a.first_tiles + tile) * a.pieces + piece
+                         : heads * a.first_tiles * a.pieces + (bh * rest + tile - a.first_tiles) * a.rest_pieces + piece;
+  return (at * 2 + which) * (kRows * 128);
+}
+
 template <bool kDk>
-__device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item &it, int piece, DkdvLds &lds) {
+__device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item &it, int piece, int pieces, DkdvLds &lds) {
   using L = DualLayout;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -869,8 +881,8 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
   // Stages t_a .. t_a + n - 1 are this piece's: kQStage rows of a head, head after head.
   const int per_head = j1 >= j0 && i_b > i_a ? (i_b - i_a + kQStage - 1) / kQStage : 0;
   const int64_t stages = (int64_t)per_head * a.rep;
-  const int64_t t_a = piece < 0 ? 0 : stages * piece / a.pieces;
-  const int n = (int)((piece < 0 ? stages : stages * (piece + 1) / a.pieces) - t_a);
+  const int64_t t_a = stages * piece / pieces;
+  const int n = (int)(stages * (piece + 1) / pieces - t_a);
   if (n > 0) {
     // Positions plo .. plo + span see the lane's key.
     int plo = key - a.right;
@@ -997,10 +1009,8 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
     return sum;
   };
   const uint32_t spoiled = n > 0 ? spoiled_columns(acc, key < sp.len) : 0;
-  if (piece >= 0) {
-    const int64_t bh = (int64_t)it.b * a.Hkv + it.h;
-    float *part = a.part + (((bh * a.first_tiles + it.tile) * a.pieces + piece) * 2 + (kDk ? 0 : 1)) * (kRows * 128) +
-                  32 * wave * 128;
+  if (pieces > 1) {
+    float *part = a.part + part_slot(a, it.b * a.Hkv + it.h, it.tile, piece, kDk ? 0 : 1) + 32 * wave * 128;
     if (!(spoiled >> l32 & 1)) {
       float *p = part + l32 * 128 + 4 * g;
 #pragma unroll
@@ -1008,7 +1018,8 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
 #pragma unroll
         for (int rr = 0; rr < 4; ++rr)
           *(float4 *)(p + dt * 32 + 8 * rr) =
-              float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]};
+              key < sp.len ? float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]}
+                           : float4{0.f, 0.f, 0.f, 0.f};
     }
     for (uint32_t left = spoiled; left; left &= left - 1) {
       const int c = __builtin_ctz(left);
@@ -1032,7 +1043,7 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
 
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dkdv_kernel(WindowArgs a) {
   __shared__ __attribute__((aligned(16))) DkdvLds lds;
-  // The grid: the whole tiles, then the pieces; each run of tiles once for dK and then
+  // The grid: the window's tiles, then the first keys'; each run of tiles once for dK and then
   // for dV, which read the same rows.
   int i = (int)blockIdx.x;
   const bool whole = i < 2 * a.grid_whole;
@@ -1040,33 +1051,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int chunk = whole ? a.chunk : a.chunk_pieces, k = i >> 3;
   const bool dv = (k / chunk) & 1;
   i = ((k / (2 * chunk) * chunk + k % chunk) << 3) | (i & 7);  // without the dK, dV pairing
-  Item it = whole ? item_of(a, i, chunk, a.nkt - a.first_tiles, a.Hkv)
-                  : item_of(a, i, chunk, a.first_tiles * a.pieces, a.Hkv);
+  const int pieces = whole ? a.rest_pieces : a.pieces;
+  Item it = item_of(a, i, chunk, (whole ? a.nkt - a.first_tiles : a.first_tiles) * pieces, a.Hkv);
   if (it.tile < 0) return;
-  int piece = -1;  // of tile it.tile
-  if (whole) {
-    it.tile += a.first_tiles;
-  } else {
-    piece = it.tile % a.pieces;
-    it.tile /= a.pieces;
-  }
-  if (dv) window_key_sums<false>(a, it, piece, lds);
-  else window_key_sums<true>(a, it, piece, lds);
+  const int piece = it.tile % pieces;
+  it.tile = it.tile / pieces + (whole ? a.first_tiles : 0);
+  if (dv) window_key_sums<false>(a, it, piece, pieces, lds);
+  else window_key_sums<true>(a, it, piece, pieces, lds);
 }
 
 // dK and dV of the tiles that were cut: the pieces' partial sums in order.  A thread
 // takes 4 dims of a key.
 __global__ void __launch_bounds__(256) window_dkdv_sum_kernel(WindowArgs a) {
-  const int rows = a.first_tiles * kRows, d = 4 * (threadIdx.x & 31);
+  const int rows = (a.rest_pieces > 1 ? a.nkt : a.first_tiles) * kRows, d = 4 * (threadIdx.x & 31);
   const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // ((b, h), dk or dv, key)
   const int key = (int)(item % rows), which = (int)(item / rows & 1);
   const int64_t bh = item / rows / 2;
   if (key >= a.Skv || bh >= (int64_t)a.B * a.Hkv) return;
   const int b = (int)(bh / a.Hkv), h = (int)(bh % a.Hkv);
-  const float *p = a.part + ((bh * a.first_tiles + key / kRows) * a.pieces * 2 + which) * (kRows * 128) +
-                   (key % kRows) * 128 + d;
+  const int tile = key / kRows, pieces = tile < a.first_tiles ? a.pieces : a.rest_pieces;
+  const float *p = a.part + part_slot(a, (int)bh, tile, 0, which) + (key % kRows) * 128 + d;
   float4 sum = *(const float4 *)p;
-  for (int i = 1; i < a.pieces; ++i) {
+  for (int i = 1; i < pieces; ++i) {
     const float4 x = *(const float4 *)(p + (int64_t)i * 2 * kRows * 128);
     sum.x += x.x;
     sum.y += x.y;
@@ -1082,7 +1088,10 @@ __global__ void __launch_bounds__(256) window_dkdv_sum_kernel(WindowArgs a) {
 // Tiles that hold first keys, and the runs each is cut into: as many as make a run no
 // longer than a window tile's, or than a quarter of what one of the chip's 512 places for
 // workgroups has to do in all, if that is more (it also bounds the partial sums: at most
-// about 1024 runs of 128 KB).  In stages of one query head.
+// about 1024 runs of 128 KB).  In stages of one query head.  Then, if the tiles' dK and dV
+// fill less than half of the places, all of them may be cut into more runs, of four stages
+// at least: the join costs about four stages, and ten if 512 runs leave partial sums
+// (H=8/1 S=1568, 119 and 26 keys to the sides: 82 us in 26 workgroups, 27 with the join).
 static void plan_dkdv(WindowArgs &a) {
   a.nkt = (a.Skv + kRows - 1) / kRows;
   a.first_tiles = (a.sinks + kRows - 1) / kRows;
@@ -1096,6 +1105,17 @@ static void plan_dkdv(WindowArgs &a) {
     a.first_tiles = 0;
     a.pieces = 1;
   }
+  const int64_t items = 2 * heads * ((int64_t)a.first_tiles * a.pieces + a.nkt - a.first_tiles);
+  int64_t best = run * a.rep;
+  a.rest_pieces = 1;
+  for (int64_t p = 2; p * items <= 512 && p * 4 <= run * a.rep; ++p) {
+    const int64_t cost = (run * a.rep + p - 1) / p + 4 + 10 * items * p / 512;
+    if (cost < best) {
+      best = cost;
+      a.rest_pieces = (int)p;
+    }
+  }
+  a.pieces *= a.rest_pieces;
 }
 
 // Rows of each of the two statistics, padded to 256 bytes.
@@ -1103,7 +1123,9 @@ static size_t stat_rows(const WindowArgs &a) { return ((size_t)a.B * a.H * a.Sq 
 
 size_t window_bwd_bytes(WindowArgs a) {
   plan_dkdv(a);
-  return 2 * stat_rows(a) * sizeof(float) + (size_t)a.B * a.Hkv * a.first_tiles * a.pieces * 2 * kRows * 128 * sizeof(float);
+  const size_t cut = (size_t)a.first_tiles * a.pieces +
+                     (a.rest_pieces > 1 ? (size_t)(a.nkt - a.first_tiles) * a.rest_pieces : 0);
+  return (2 * stat_rows(a) + (size_t)a.B * a.Hkv * cut * 2 * kRows * 128) * sizeof(float);
 }
 
 // Grid of `tiles` work items for each of a batch's `heads` heads (item_of).  Runs are as long
@@ -1202,12 +1224,12 @@ int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s) {
   if (rc) return rc;
   plan_dkdv(a);
   a.part = a.stats + 2 * a.stats_n;
-  a.grid_whole = deal(a, a.nkt - a.first_tiles, a.Hkv, 128, &a.chunk);
+  a.grid_whole = deal(a, (a.nkt - a.first_tiles) * a.rest_pieces, a.Hkv, 128, &a.chunk);
   a.grid_pieces = deal(a, a.first_tiles * a.pieces, a.Hkv, 128, &a.chunk_pieces);
   hipLaunchKernelGGL(window_dkdv_kernel, dim3((unsigned)(2 * a.grid_whole + 2 * a.grid_pieces)), dim3(256), 0, s, a);
   rc = check_launch("window_dkdv_kernel");
-  if (rc || a.first_tiles == 0) return rc;
-  const int64_t rows = (int64_t)a.B * a.Hkv * a.first_tiles * kRows * 2;
+  if (rc || (a.first_tiles == 0 && a.rest_pieces == 1)) return rc;
+  const int64_t rows = (int64_t)a.B * a.Hkv * (a.rest_pieces > 1 ? a.nkt : a.first_tiles) * kRows * 2;
   hipLaunchKernelGGL(window_dkdv_sum_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a);
   return check_launch("window_dkdv_sum_kernel");
 }

@@ -303,3 +303,11 @@ def test_stream_and_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.parametrize("H,Hkv,S,window,sinks,causal", [(8, 1, 600, (119, 26), 0, False), (14, 2, 513, (67, 0), 50, True),
+                                                         (6, 1, 200, (300, 300), 0, False), (4, 1, 130, (3, 2), 129, False)])
+def test_few_key_tiles(gpu, H, Hkv, S, window, sinks, causal):
+    # Too few tiles to fill the chip: all of them cut into runs of queries, ragged ones too.
+    check(gpu, 1, H, Hkv, S, S, window, sinks, causal, seed=S)
+    check(gpu, 2, H, Hkv, S, S, window, sinks, causal, kv_lens=[S, S // 3], q_start=[0, 0], seed=S + 1)
