@@ -117,6 +117,14 @@ def qk_rmsnorm_rope_axes(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, ax
     return oq, ok
 
 
+@functools.lru_cache(maxsize=256)
+def _rope_bwd_bytes(B: int, S: int) -> int:
+    n = ctypes.c_size_t(0)
+    check("h3a_qk_rmsnorm_rope_axes_bwd_workspace_size",
+          lib().h3a_qk_rmsnorm_rope_axes_bwd_workspace_size(B, S, ctypes.byref(n)))
+    return n.value
+
+
 def qk_rmsnorm_rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor,
                              axes, qw: torch.Tensor, kw: torch.Tensor, eps: float = 1e-6, theta: float = 10000.0):
     """Gradients of qk_rmsnorm_rope_axes from those of its outputs: (q's, k's, qw's, kw's).
@@ -131,18 +139,16 @@ def qk_rmsnorm_rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor
     dk, dkst = _rope_input("dk", dk, q.device)
     gq, gqst = _rope_output("dq", None, q.shape, q.device)
     gk, gkst = _rope_output("dk", None, k.shape, q.device)
-    gw = torch.empty((2, D), dtype=torch.float32, device=q.device)
+    gqw, gkw = (torch.empty(D, dtype=torch.float32, device=q.device) for _ in range(2))
+    nbytes = _rope_bwd_bytes(B, S)
     with _on_device(q):
-        n = ctypes.c_size_t(0)
-        check("h3a_qk_rmsnorm_rope_axes_bwd_workspace_size",
-              lib().h3a_qk_rmsnorm_rope_axes_bwd_workspace_size(B, S, ctypes.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib().h3a_qk_rmsnorm_rope_axes_bwd(dq.data_ptr(), dk.data_ptr(), q.data_ptr(), k.data_ptr(), gq.data_ptr(),
-                                                gk.data_ptr(), gw[0].data_ptr(), gw[1].data_ptr(), B, S, Hq, Hk, D,
+                                                gk.data_ptr(), gqw.data_ptr(), gkw.data_ptr(), B, S, Hq, Hk, D,
                                                 dqst, dkst, qst, kst, gqst, gkst, ctypes.byref(p), qw.data_ptr(),
-                                                kw.data_ptr(), float(eps), ws.data_ptr(), n.value, _stream(q))
+                                                kw.data_ptr(), float(eps), ws.data_ptr(), nbytes, _stream(q))
     check("h3a_qk_rmsnorm_rope_axes_bwd", rc)
-    return gq, gk, gw[0], gw[1]
+    return gq, gk, gqw, gkw
 
 
 # ---------------------------------------------------------------------------
@@ -163,6 +169,15 @@ def _bounds(segments, rows: int, groups):
     if groups is not None and groups != len(segments) - 1:
         raise ValueError(f"{len(segments) - 1} segments, but weights for {groups}")
     return (ctypes.c_int * len(segments))(*segments)
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_bwd_bytes(split: tuple, C: int) -> int:
+    """Workspace bytes of the weights' gradients; split: the arguments of _bounds."""
+    bounds, n = _bounds(*split), ctypes.c_size_t(0)
+    check("h3a_layer_norm_bwd_workspace_size",
+          lib().h3a_layer_norm_bwd_workspace_size(bounds, len(bounds) - 1, C, ctypes.byref(n)))
+    return n.value
 
 
 def _norm_rows(name: str, t: torch.Tensor, C: int) -> torch.Tensor:
@@ -195,10 +210,10 @@ def _norm_prepare(x, weight, bias, segments):
         if groups is not None and n != groups:
             raise ValueError("weight and bias must have the same segments")
         groups = n
-    bounds = _bounds(None if segments is None else whole_numbers("segments", segments), rows, groups)
+    split = (None if segments is None else whole_numbers("segments", segments), rows, groups)
     dt = DTYPES[affine[0][1].dtype] if affine else _lib.FP32
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    return rows, C, bounds, dt, weight, bias
+    return rows, C, split, _bounds(*split), dt, weight, bias
 
 
 def _ptr(t):
@@ -216,17 +231,17 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     16384; weight and bias any of these.  Returns y, with return_stats (y, mean, rstd),
     the fp32 [rows] statistics that layer_norm_bwd takes.
     """
-    rows, C, bounds, dt, weight, bias = _norm_prepare(x, weight, bias, segments)
+    rows, C, _, bounds, dt, weight, bias = _norm_prepare(x, weight, bias, segments)
     x2 = _norm_rows("x", x, C)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
+    mean, rstd = (torch.empty(rows, dtype=torch.float32, device=x.device) if return_stats else None for _ in range(2))
     with _on_device(x):
         rc = lib().h3a_layer_norm_fwd(x2.data_ptr(), x2.stride(0), _ptr(weight), _ptr(bias), y.data_ptr(), C,
-                                      _ptr(stats), None if stats is None else stats[1].data_ptr(), rows, C,
+                                      _ptr(mean), _ptr(rstd), rows, C,
                                       DTYPES[x.dtype], dt, bounds, len(bounds) - 1, 1 if modulate else 0,
                                       float(eps), _stream(x))
     check("h3a_layer_norm_fwd", rc)
-    return (y, stats[0], stats[1]) if return_stats else y
+    return (y, mean, rstd) if return_stats else y
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, mean: torch.Tensor,
@@ -237,7 +252,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
     a fixed order, [C], or [n, C] where weight is or segments are given; None without
     param_grads.
     """
-    rows, C, bounds, dt, weight, _ = _norm_prepare(x, weight, None, segments)
+    rows, C, split, bounds, dt, weight, _ = _norm_prepare(x, weight, None, segments)
     if not isinstance(dy, torch.Tensor) or dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("dy must be a tensor like x")
     for name, t in (("mean", mean), ("rstd", rstd)):
@@ -246,19 +261,17 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
     x2, dy2 = _norm_rows("x", x, C), _norm_rows("dy", dy, C)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     n = len(bounds) - 1
-    grads, ws, nbytes = None, None, ctypes.c_size_t(0)
+    dw = db = ws = None
+    nbytes = 0
     with _on_device(x):
         if param_grads:
-            grads = torch.empty((2, n, C), dtype=torch.float32, device=x.device)
-            check("h3a_layer_norm_bwd_workspace_size",
-                  lib().h3a_layer_norm_bwd_workspace_size(bounds, n, C, ctypes.byref(nbytes)))
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
+            shape = C if n == 1 and (weight is None or weight.dim() == 1) else (n, C)
+            dw, db = (torch.empty(shape, dtype=torch.float32, device=x.device) for _ in range(2))
+            nbytes = _norm_bwd_bytes(split, C)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         rc = lib().h3a_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(weight),
-                                      mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), C, _ptr(grads),
-                                      None if grads is None else grads[1].data_ptr(), rows, C, DTYPES[x.dtype], dt,
-                                      bounds, n, 1 if modulate else 0, _ptr(ws), nbytes.value, _stream(x))
+                                      mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), C, _ptr(dw), _ptr(db), rows, C,
+                                      DTYPES[x.dtype], dt, bounds, n, 1 if modulate else 0, _ptr(ws), nbytes,
+                                      _stream(x))
     check("h3a_layer_norm_bwd", rc)
-    if grads is None:
-        return dx, None, None
-    flat = n == 1 and (weight is None or weight.dim() == 1)
-    return dx, grads[0, 0] if flat else grads[0], grads[1, 0] if flat else grads[1]
+    return dx, dw, db
