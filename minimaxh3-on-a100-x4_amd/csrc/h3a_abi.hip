@@ -572,7 +572,8 @@ int h3a_attn_fwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, i
   if (rc) return rc;
   WindowArgs a;
   fill_window_args(a, B, H, Hkv, Sq, Skv, *window, 1.f);
-  return window_fwd_bytes(a, bytes);
+  bool split;
+  return plan_window_fwd(a, &split, bytes);
 }
 
 int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, float *lse, int B, int H, int Hkv,
@@ -600,12 +601,13 @@ int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, fl
   put_strides(a.vsb, a.vsh, a.vss, v_strides, Skv);
   put_strides(a.osb, a.osh, a.oss, o_strides, Sq);
   size_t need = 0;
-  rc = window_fwd_bytes(a, &need);
+  bool split;
+  rc = plan_window_fwd(a, &split, &need);
   if (rc) return rc;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(H3A_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
   if (need > 0 && !aligned16(workspace)) return fail(H3A_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  return launch_window_fwd(a, workspace, as_stream(stream));
+  return launch_window_fwd(a, split, workspace, as_stream(stream));
 }
 
 int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D, const h3a_window *window,

@@ -148,8 +148,9 @@ struct WindowArgs {
   int rest_pieces;          // runs of each other tile (1: not cut)
   float *part;              // the runs' partial sums, [..][dK, dV][128][128] (part_slot)
 };
-int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s);
-int window_fwd_bytes(WindowArgs a, size_t *bytes);  // workspace on the current device
+// Whether the current device takes the keys in pieces (a.nqt, a.pieces), and the workspace.
+int plan_window_fwd(WindowArgs &a, bool *split, size_t *bytes);
+int launch_window_fwd(WindowArgs a, bool split, void *ws, hipStream_t s);
 int launch_window_bwd(WindowArgs a, void *ws, hipStream_t s);
 size_t window_bwd_bytes(WindowArgs a);  // workspace, from the sizes and the window
 

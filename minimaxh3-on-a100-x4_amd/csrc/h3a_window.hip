@@ -1185,21 +1185,20 @@ static int cu_count(int *cus) {
   return H3A_OK;
 }
 
-int window_fwd_bytes(WindowArgs a, size_t *bytes) {
+int plan_window_fwd(WindowArgs &a, bool *split, size_t *bytes) {
+  *split = false;
   *bytes = 0;
   if (a.Sq > kTokenMaxRows) return H3A_OK;
   int cus = 0;
   const int rc = cu_count(&cus);
   if (rc) return rc;
-  if (plan_token(a, cus) && a.pieces > 1) *bytes = (size_t)a.B * a.Hkv * a.nqt * a.pieces * kTokenRows * (128 + 2) * sizeof(float);
+  *split = plan_token(a, cus);
+  if (*split && a.pieces > 1) *bytes = (size_t)a.B * a.Hkv * a.nqt * a.pieces * kTokenRows * (128 + 2) * sizeof(float);
   return H3A_OK;
 }
 
-int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
-  int cus = 0;
-  int rc = a.Sq <= kTokenMaxRows ? cu_count(&cus) : H3A_OK;
-  if (rc) return rc;
-  if (!plan_token(a, cus)) {
+int launch_window_fwd(WindowArgs a, bool split, void *ws, hipStream_t s) {
+  if (!split) {
     a.nqt = (a.Sq + kRows - 1) / kRows;
     const int grid = deal(a, a.nqt, a.H, 256, &a.chunk);
     hipLaunchKernelGGL(window_fwd_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
@@ -1208,7 +1207,7 @@ int launch_window_fwd(WindowArgs a, void *ws, hipStream_t s) {
   a.part = static_cast<float *>(ws);
   const int units = a.B * a.Hkv * a.nqt;
   hipLaunchKernelGGL(window_token_kernel, dim3((unsigned)(units * a.pieces)), dim3(256), 0, s, a);
-  rc = check_launch("window_token_kernel");
+  const int rc = check_launch("window_token_kernel");
   if (rc || a.pieces == 1) return rc;
   hipLaunchKernelGGL(window_token_sum_kernel, dim3((unsigned)(units * kTokenRows)), dim3(256), 0, s, a, units);
   return check_launch("window_token_sum_kernel");

@@ -45,6 +45,8 @@ def mask_args(window, sinks):
     if not isinstance(window, (tuple, list)) or len(window) != 2:
         raise ValueError(f"window must be a pair (left, right), got {window!r}")
     left, right = window
+    if type(left) is int and type(right) is int and type(sinks) is int:
+        return (left, right), sinks
     if type(left) is not int and left is not None:
         left = _whole("window's left side", left)
     if type(right) is not int and right is not None:

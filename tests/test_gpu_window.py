@@ -311,3 +311,27 @@ def test_few_key_tiles(gpu, H, Hkv, S, window, sinks, causal):
     # Too few tiles to fill the chip: all of them cut into runs of queries, ragged ones too.
     check(gpu, 1, H, Hkv, S, S, window, sinks, causal, seed=S)
     check(gpu, 2, H, Hkv, S, S, window, sinks, causal, kv_lens=[S, S // 3], q_start=[0, 0], seed=S + 1)
+
+
+def test_calls_at_once_on_two_streams(gpu):
+    """Split keys and cut tiles leave partial results in workspaces: each call has its own."""
+    sets = [make(gpu, 1, 8, 1, 300, 300, seed) for seed in (1, 2)]
+    kw = dict(window=(40, 30), sinks=140)
+
+    def step(q, k, v, do):
+        one = h3attn.attn_fwd_window(q[:, :, -1:], k, v, **kw)
+        o, lse = h3attn.attn_fwd_window(q, k, v, return_lse=True, **kw)
+        return (one, o, lse, *h3attn.attn_bwd_window(do, q, k, v, o, lse, **kw))
+
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(want[i], g))
