@@ -19,7 +19,6 @@ heads are a rank's share when 2 or 4 GPUs split the heads.
 """
 from __future__ import annotations
 
-import functools
 import math
 import os
 import sys
@@ -35,9 +34,8 @@ FULL_S, FULL_H, FULL_C = 42120, 56, 5376
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
-@functools.lru_cache(maxsize=None)
 def _h3attn():
-    """The package under test; only looked up where `own` is true, and once, as a program imports it."""
+    """The package under test; only looked up where `own` is true."""
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "minimaxh3-on-a100-x4_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
