@@ -92,19 +92,23 @@ __device__ __forceinline__ u32x4 buffer_load_b128(__amdgpu_buffer_rsrc_t res, ui
 // after one of its loads only make a wait for that load more conservative.
 // `desc` is the V# as four scalar words (stage_desc); `m0` is the LDS byte
 // address of the destination (lds_address).
+// The load reads M0 one wait state after a scalar instruction wrote it at the earliest, and
+// the compiler, which copies m0 there right before, keeps that distance to its own loads
+// only: the s_nop (dense and block-sparse at S=42120: no change to 0.8 % of the time).
 __device__ __forceinline__ void buffer_load_lds_b128(u32x4 desc, uint32_t byte_off, uint32_t m0) {
-  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(byte_off), "s"(desc), "{m0}"(m0)
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(byte_off), "s"(desc), "{m0}"(m0)
                : "memory");
 }
 
 // The same for 4 bytes per lane: to lds_dst + 4 * lane.
 __device__ __forceinline__ void buffer_load_lds_b32(u32x4 desc, uint32_t byte_off, uint32_t m0) {
-  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(byte_off), "s"(desc), "{m0}"(m0) : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(byte_off), "s"(desc), "{m0}"(m0)
+               : "memory");
 }
 
 // The same from a 64-bit address per lane, with no range check.
 __device__ __forceinline__ void global_load_lds_b128(const void *p, uint32_t m0) {
-  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(m0) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(m0) : "memory");
 }
 
 // LDS byte address of a pointer into a __shared__ array.
@@ -122,26 +126,6 @@ __device__ __forceinline__ uint32_t opaque_sadd(uint32_t x) {
   return r;
 }
 
-// stage_rsrc's V# as four words for inline asm: base address (48 bits, stride
-// 0), num_records, config.  Each word goes through readfirstlane, so the
-// operand is provably wave-uniform and lives in SGPRs whatever the register
-// pressure around the call.
-__device__ __forceinline__ u32x4 stage_desc(const uint16_t *base, int64_t stride, int rows) {
-  const uint32_t bytes = stage_bytes(stride, rows);
-  const uint64_t addr = reinterpret_cast<uint64_t>(base);
-  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xffffu)),
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufferConfig};
-}
-
-// The V# of `bytes` bytes from p (wave-uniform).
-__device__ __forceinline__ u32x4 range_desc(const void *p, int bytes) {
-  const uint64_t addr = reinterpret_cast<uint64_t>(p);
-  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xffffu)),
-               (uint32_t)__builtin_amdgcn_readfirstlane(bytes), (uint32_t)kBufferConfig};
-}
-
 // A descriptor ready for the inline-asm loads above.  A vector instruction's scalar
 // result (readfirstlane) may be read by a vector-memory instruction five wait states
 // later at the earliest; the compiler keeps that distance to its own loads only, and a
@@ -149,6 +133,26 @@ __device__ __forceinline__ u32x4 range_desc(const void *p, int bytes) {
 __device__ __forceinline__ u32x4 settled(u32x4 desc) {
   asm volatile("s_nop 4" : "+s"(desc));
   return desc;
+}
+
+// stage_rsrc's V# as four words for inline asm: base address (48 bits, stride
+// 0), num_records, config.  Each word goes through readfirstlane, so the
+// operand is provably wave-uniform and lives in SGPRs whatever the register
+// pressure around the call.
+__device__ __forceinline__ u32x4 stage_desc(const uint16_t *base, int64_t stride, int rows) {
+  const uint32_t bytes = stage_bytes(stride, rows);
+  const uint64_t addr = reinterpret_cast<uint64_t>(base);
+  return settled(u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xffffu)),
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufferConfig});
+}
+
+// The V# of `bytes` bytes from p (wave-uniform).
+__device__ __forceinline__ u32x4 range_desc(const void *p, int bytes) {
+  const uint64_t addr = reinterpret_cast<uint64_t>(p);
+  return settled(u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(addr >> 32) & 0xffffu)),
+                       (uint32_t)__builtin_amdgcn_readfirstlane(bytes), (uint32_t)kBufferConfig});
 }
 
 // s_waitcnt vmcnt(N): at most the N most recent vector-memory loads of this

@@ -206,6 +206,7 @@ struct StageCursor {
     step_hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(step >> 32));
     ss2 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(ss * 2));
     rows_left = __builtin_amdgcn_readfirstlane(key_end - key0);
+    asm volatile("s_nop 4" : "+s"(lo), "+s"(hi), "+s"(ss2), "+s"(rows_left));  // as settled()
   }
   // The V# of the current stage, as stage_desc builds it: valid rows only.
   __device__ __forceinline__ u32x4 desc() const {

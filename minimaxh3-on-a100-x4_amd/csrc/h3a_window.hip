@@ -261,7 +261,7 @@ __device__ __forceinline__ float lane_value(float x, int lane) {
 template <class Dma>
 __device__ __forceinline__ void fetch_tile(const Dma &dma, const uint16_t *base, int64_t stride, int row0, int limit,
                                            uint16_t *tile) {
-  dma.template issue_desc<0, Dma::kInst>(settled(dma.desc(base, stride, row0, limit)), tile);
+  dma.template issue_desc<0, Dma::kInst>(dma.desc(base, stride, row0, limit), tile);
 }
 
 // A sequence of the batch: first query's position, keys, and the rows that are tokens.
@@ -905,7 +905,7 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
       if (wave < (kDk ? 2 : 1)) {
         const int rows = i_b - frow < kQStage ? i_b - frow : kQStage;
         const float *st = a.stats + wave * a.stats_n + ((int64_t)it.b * a.H + fh) * a.Sq + frow;
-        buffer_load_lds_b32(settled(range_desc(st, rows * 4)), 4 * lane, lds_address(lds.stats[slot][wave]));
+        buffer_load_lds_b32(range_desc(st, rows * 4), 4 * lane, lds_address(lds.stats[slot][wave]));
       }
       frow += kQStage;
       if (frow >= i_b) {
