@@ -266,7 +266,8 @@ int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, fl
  * the forward's o and lse; dk and dv are sums over the heads that share a key
  * head.  Rows that belong to no token get dq = 0 and give no gradient, keys at or
  * past len get dk = dv = 0.  The sums run in a fixed order: equal calls give equal
- * bits.  workspace: h3a_attn_bwd_window_workspace_size bytes, untouched until the
+ * bits.  Unlike the forward's, the sequence strides of dout and q are a row (D
+ * elements) or more, as a written tensor's.  workspace: h3a_attn_bwd_window_workspace_size bytes, untouched until the
  * call's work has completed.
  */
 int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, int D,

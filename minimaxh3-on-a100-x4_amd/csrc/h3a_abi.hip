@@ -169,14 +169,16 @@ int check_window(const h3a_window *w, int Sq, int Skv, float scale) {
   return H3A_OK;
 }
 
-// One tensor of S rows: pointer, strides; written ones must not overlap themselves.
-int check_rows(const char *name, const void *p, const int64_t *st, int S, bool written) {
+// One tensor of S rows: pointer, strides.  `apart`: rows may not overlap, being written, or
+// fetched in stages whose rows past the sequence's end have to arrive as zeros (stage_bytes:
+// the range ends with the last row, which closer rows past it would still lie in).
+int check_rows(const char *name, const void *p, const int64_t *st, int S, bool apart) {
   if (!p || !st) return fail(H3A_ERR_INVALID_ARG, "%s: null pointer or strides", name);
   if (!aligned16(p)) return fail(H3A_ERR_ALIGNMENT, "%s must be 16-byte aligned", name);
   if (!strides_ok(st)) return fail(H3A_ERR_ALIGNMENT, "%s strides must be non-negative multiples of 8 elements", name);
   if (S > 1 && st[2] >= kMaxSeqStride)
     return fail(H3A_ERR_UNSUPPORTED, "%s sequence stride must be < %lld elements", name, (long long)kMaxSeqStride);
-  if (written && S > 1 && st[2] < kRowElems)
+  if (apart && S > 1 && st[2] < kRowElems)
     return fail(H3A_ERR_INVALID_ARG, "%s sequence stride %lld is less than a row (%lld elements): rows overlap", name,
                 (long long)st[2], (long long)kRowElems);
   return H3A_OK;
@@ -633,8 +635,8 @@ int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const vo
   clear_error();
   int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
   if (!rc) rc = check_window(window, Sq, Skv, scale);
-  if (!rc) rc = check_rows("dout", dout, dout_strides, Sq, false);
-  if (!rc) rc = check_rows("q", q, q_strides, Sq, false);
+  if (!rc) rc = check_rows("dout", dout, dout_strides, Sq, true);
+  if (!rc) rc = check_rows("q", q, q_strides, Sq, true);
   if (!rc) rc = check_rows("k", k, k_strides, Skv, false);
   if (!rc) rc = check_rows("v", v, v_strides, Skv, false);
   if (!rc) rc = check_rows("o", o, o_strides, Sq, false);

@@ -162,6 +162,14 @@ def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, s
     return (out, lse) if return_lse else out
 
 
+def _rows_apart(name: str, t: torch.Tensor):
+    """t and its strides with rows that do not overlap, copied where they do (a gradient expanded over the sequence)."""
+    t, st = _as_kernel_input(name, t)
+    if t.shape[2] > 1 and st[2] < HEAD_DIM:
+        t, st = _as_kernel_input(name, t.contiguous())
+    return t, st
+
+
 def _grad_like(t: torch.Tensor):
     """A tensor for t's gradient, in t's order of dimensions where the kernels can write it."""
     g = torch.empty_like(t)
@@ -183,7 +191,8 @@ def attn_bwd_window(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     q, k, v, (B, H, Hkv, Sq, Skv, D), st = _prepare(q, k, v)
     _check_like("dout", dout, q)
     _check_like("o", o, q)
-    dout, gst = _as_kernel_input("dout", dout)
+    q, qst = _rows_apart("q", q)
+    dout, gst = _rows_apart("dout", dout)
     o, ost = _as_kernel_input("o", o)
     if lse.shape != (B, H, Sq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise ValueError(f"lse must be the forward's fp32 [{B},{H},{Sq}] tensor")
@@ -195,7 +204,7 @@ def attn_bwd_window(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib().h3a_attn_bwd_window(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                        lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Sq,
-                                       Skv, D, gst, *st, ost, dqst, dkst, dvst, ctypes.byref(w), sc, ws.data_ptr(),
+                                       Skv, D, gst, qst, *st[1:], ost, dqst, dkst, dvst, ctypes.byref(w), sc, ws.data_ptr(),
                                        nbytes, _stream(q))
     check("h3a_attn_bwd_window", rc)
     return dq, dk, dv

@@ -1,0 +1,42 @@
+"""Windowed attention on the GPU: calls that the documentation allows and that are easily got wrong."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import h3attn
+import window_ref as ref
+from h3attn import autograd
+from test_gpu_window import SCALE, check, close, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B,H,Hkv,S,window,sinks,lens", [(1, 2, 2, 40, (None, None), 0, None), (2, 4, 2, 200, (30, 30), 9, None),
+                                                         (2, 4, 2, 200, (30, 30), 140, [150, 70]),
+                                                         (3, 40, 8, 170, (20, 200), 0, [170, 3, 99])])
+@pytest.mark.parametrize("which", ["dout", "q", "both", "overlapping"])
+def test_rows_that_share_memory(gpu, B, H, Hkv, S, window, sinks, lens, which):
+    """A gradient expanded over the sequence (that of a mean over it), one query for all rows, overlapping rows."""
+    q, k, v, do = make(gpu, B, H, Hkv, S, S, seed=S)
+    wide = lambda t: t[:, :, :1].expand(B, H, S, 128)  # noqa: E731
+    if which == "overlapping":
+        mem = do.contiguous().view(B, H, S * 128)
+        do = mem.as_strided((B, H, S, 128), (H * S * 128, S * 128, 64, 1))
+    else:
+        do = wide(do) if which != "q" else do
+        q = wide(q) if which != "dout" else q
+    check(gpu, B, H, Hkv, S, S, window, sinks, kv_lens=lens, tensors=(q, k, v, do))
+
+
+def test_gradient_of_a_mean_over_the_sequence(gpu):
+    B, H, S = 1, 3, 150
+    q, k, v, _ = (t.detach().requires_grad_() for t in make(gpu, B, H, H, S, S, seed=1))
+    o = autograd.window_attention(q, k, v, (25, 25), sinks=5)
+    o.sum(dim=2).backward(g := torch.ones(B, H, 128, dtype=torch.bfloat16, device=gpu))
+    do = g[:, :, None].expand(B, H, S, 128).cpu()
+    c = [t.detach().cpu() for t in (q, k, v)]
+    mask = ref.visible(B, S, S, (25, 25), 5, False, None, None)
+    for name, t, w, b in zip(("dq", "dk", "dv"), (q, k, v), ref.backward(do, *c, mask, SCALE),
+                             ref.backward_bounds(do, *c, mask, SCALE)):
+        close(t.grad, w, b, name)
