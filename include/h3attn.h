@@ -238,7 +238,8 @@ typedef struct {
   int left, right;          /* keys seen to either side of a position, >= 0 */
   int sinks;                /* first keys seen from every position, >= 0 */
   int causal;               /* no key past the position (right and sinks included) */
-  int q_start;              /* position of row 0; 0 <= q_start <= Skv - Sq unless q_starts is given */
+  int q_start;              /* position of row 0; 0 <= q_start <= Skv - Sq unless q_starts is given
+                             (a workspace's size does not depend on either) */
   const int32_t *q_starts;  /* [B] on the device, or NULL */
   const int32_t *kv_lens;   /* [B] on the device, or NULL: Skv keys */
 } h3a_window;

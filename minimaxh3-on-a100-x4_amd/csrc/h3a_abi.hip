@@ -154,11 +154,19 @@ int check_window_sizes(int B, int H, int Hkv, int Sq, int Skv, int D) {
   return H3A_OK;
 }
 
-int check_window(const h3a_window *w, int Sq, int Skv, float scale) {
+// What a workspace's size depends on.
+int check_window(const h3a_window *w) {
   if (!w) return fail(H3A_ERR_INVALID_ARG, "null window");
   if (w->left < 0 || w->right < 0 || w->sinks < 0)
     return fail(H3A_ERR_INVALID_ARG, "window sides and sinks must not be negative (left=%d right=%d sinks=%d)", w->left,
                 w->right, w->sinks);
+  return H3A_OK;
+}
+
+// And a launch beside it.
+int check_window_call(const h3a_window *w, int Sq, int Skv, float scale) {
+  const int rc = check_window(w);
+  if (rc) return rc;
   if (!w->q_starts && (w->q_start < 0 || w->q_start > Skv - Sq))
     return fail(H3A_ERR_INVALID_ARG, "q_start %d: rows must lie at positions 0 .. Skv - 1 (Sq=%d Skv=%d)", w->q_start,
                 Sq, Skv);
@@ -570,7 +578,7 @@ int h3a_attn_fwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, i
   clear_error();
   if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
   int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
-  if (!rc) rc = check_window(window, Sq, Skv, 1.f);
+  if (!rc) rc = check_window(window);
   if (rc) return rc;
   WindowArgs a;
   fill_window_args(a, B, H, Hkv, Sq, Skv, *window, 1.f);
@@ -584,7 +592,7 @@ int h3a_attn_fwd_window(const void *q, const void *k, const void *v, void *o, fl
                         float scale, void *workspace, size_t workspace_bytes, h3a_stream_t stream) {
   clear_error();
   int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
-  if (!rc) rc = check_window(window, Sq, Skv, scale);
+  if (!rc) rc = check_window_call(window, Sq, Skv, scale);
   if (!rc) rc = check_rows("q", q, q_strides, Sq, false);
   if (!rc) rc = check_rows("k", k, k_strides, Skv, false);
   if (!rc) rc = check_rows("v", v, v_strides, Skv, false);
@@ -617,7 +625,7 @@ int h3a_attn_bwd_window_workspace_size(int B, int H, int Hkv, int Sq, int Skv, i
   clear_error();
   if (!bytes) return fail(H3A_ERR_INVALID_ARG, "null output pointer");
   int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
-  if (!rc) rc = check_window(window, Sq, Skv, 1.f);
+  if (!rc) rc = check_window(window);
   if (rc) return rc;
   WindowArgs a;
   fill_window_args(a, B, H, Hkv, Sq, Skv, *window, 1.f);
@@ -634,7 +642,7 @@ int h3a_attn_bwd_window(const void *dout, const void *q, const void *k, const vo
                         h3a_stream_t stream) {
   clear_error();
   int rc = check_window_sizes(B, H, Hkv, Sq, Skv, D);
-  if (!rc) rc = check_window(window, Sq, Skv, scale);
+  if (!rc) rc = check_window_call(window, Sq, Skv, scale);
   if (!rc) rc = check_rows("dout", dout, dout_strides, Sq, true);
   if (!rc) rc = check_rows("q", q, q_strides, Sq, true);
   if (!rc) rc = check_rows("k", k, k_strides, Skv, false);

@@ -75,7 +75,8 @@ def _sides(window, sinks, causal, start, Sq, Skv):
 
 
 def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device):
-    """The call's h3a_window, and what its workspace's size depends on."""
+    """The call's h3a_window, and its (left, right, sinks, causal, start), of which a workspace's size depends on the
+    first four."""
     window, sinks = mask_args(window, sinks)
     lens = None if kv_lens is None else _per_sequence("kv_lens", kv_lens, B, device)
     starts = None
@@ -93,8 +94,8 @@ def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device):
 
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(fn: str, sizes: tuple, sides: tuple, device_index: int) -> int:
-    """Workspace bytes of entry point fn on the device, which is the current one."""
-    left, right, sinks, causal, start = sides
+    """Workspace bytes of entry point fn on the device, which is the current one; sides: (left, right, sinks, causal)."""
+    left, right, sinks, causal = sides
     w, n = _lib.Window(left, right, sinks, causal, 0, None, None), ctypes.c_size_t(0)
     check(fn, getattr(lib(), fn)(*sizes, ctypes.byref(w), ctypes.byref(n)))
     return n.value
@@ -151,7 +152,7 @@ def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, s
     with _on_device(q):
         ws, nbytes = None, 0
         if Sq <= SPLIT_ROWS:
-            nbytes = _workspace_bytes("h3a_attn_fwd_window_workspace_size", (B, H, Hkv, Sq, Skv, D), sides,
+            nbytes = _workspace_bytes("h3a_attn_fwd_window_workspace_size", (B, H, Hkv, Sq, Skv, D), sides[:4],
                                       q.get_device())
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib().h3a_attn_fwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
@@ -200,7 +201,8 @@ def attn_bwd_window(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     (dq, dqst), (dk, dkst), (dv, dvst) = _grad_like(q), _grad_like(k), _grad_like(v)
     sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
     with _on_device(q):
-        nbytes = _workspace_bytes("h3a_attn_bwd_window_workspace_size", (B, H, Hkv, Sq, Skv, D), sides, q.get_device())
+        nbytes = _workspace_bytes("h3a_attn_bwd_window_workspace_size", (B, H, Hkv, Sq, Skv, D), sides[:4],
+                                  q.get_device())
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib().h3a_attn_bwd_window(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                        lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, H, Hkv, Sq,

@@ -40,3 +40,13 @@ def test_gradient_of_a_mean_over_the_sequence(gpu):
     for name, t, w, b in zip(("dq", "dk", "dv"), (q, k, v), ref.backward(do, *c, mask, SCALE),
                              ref.backward_bounds(do, *c, mask, SCALE)):
         close(t.grad, w, b, name)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Sq,Skv", [(2, 2, 1, 140, 100), (4, 40, 8, 300, 129), (1, 1, 1, 20, 1), (1, 1, 1, 8300, 70)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_more_rows_than_keys(gpu, B, H, Hkv, Sq, Skv, causal):
+    """Starts per sequence put a query buffer that is longer than the cache; rows outside it give zeros."""
+    starts = [0, -Sq + 30, Skv - 5, -17][:B]
+    check(gpu, B, H, Hkv, Sq, Skv, (40, 0 if causal else 25), 6, causal, q_start=starts)
+    check(gpu, B, H, Hkv, Sq, Skv, (40, 0 if causal else 25), 6, causal, q_start=starts,
+          kv_lens=[Skv - 1, Skv // 2, Skv, 0][:B])

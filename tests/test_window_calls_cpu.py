@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import ctypes
 
-from h3attn import _lib
+from h3attn import _lib, window
 
 S3 = _lib.strides3
 ROW = S3(0, 0, 128)
@@ -20,3 +20,28 @@ def test_backward_rows_apart():
             assert L.h3a_attn_bwd_window(*(16,) * 9, 1, 2, 1, 4, 4, 128, *st, ctypes.byref(w), 0.1, None, n.value,
                                          None) == _lib.H3A_ERR_INVALID_ARG
             assert name + b" sequence stride" in L.h3a_last_error()
+
+
+def test_workspace_size_knows_no_positions():
+    """Starts given per sequence may put more rows than keys; how many bytes a call needs does not depend on them."""
+    L = _lib.lib()
+    for fn in (L.h3a_attn_fwd_window_workspace_size, L.h3a_attn_bwd_window_workspace_size):
+        if fn is L.h3a_attn_fwd_window_workspace_size:
+            sizes = (1, 2, 1, 9000, 100, 128)  # (up to 8192 rows it asks the device)
+        else:
+            sizes = (1, 2, 1, 140, 100, 128)
+        got = []
+        for start, starts in ((0, None), (0, 16), (7, None)):
+            n = ctypes.c_size_t(1)
+            assert fn(*sizes, ctypes.byref(_lib.Window(3, 3, 1, 0, start, starts, None)), ctypes.byref(n)) == 0
+            got.append(n.value)
+        assert len(set(got)) == 1
+    window._workspace_bytes.cache_clear()
+    for _ in range(3):
+        window._workspace_bytes("h3a_attn_bwd_window_workspace_size", (1, 2, 1, 140, 100, 128), (3, 3, 1, 0), 0)
+    assert window._workspace_bytes.cache_info().misses == 1
+    # A launch still checks where its rows are.
+    w = _lib.Window(3, 3, 1, 0, 0, None, None)
+    assert L.h3a_attn_fwd_window(16, 16, 16, 16, None, 1, 2, 1, 140, 100, 128, *(ROW,) * 4, ctypes.byref(w), 0.1, None,
+                                 0, None) == _lib.H3A_ERR_INVALID_ARG
+    assert b"rows must lie at positions" in L.h3a_last_error()
