@@ -158,6 +158,8 @@ def _bounds(segments, rows: int, groups):
     """Checked bounds of the segments as the entry points take them; None: `groups` equal ones."""
     if rows > 2 ** 30:
         raise ValueError(f"{rows} rows unsupported (at most 2^30)")
+    if groups == 0:
+        raise ValueError("weight and bias must have a row for one segment at least")
     if segments is None:
         groups = groups or 1
         if rows % groups:
