@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from .block import layer_norm_bwd, layer_norm_fwd, qk_rmsnorm_rope_axes, qk_rmsnorm_rope_axes_bwd, whole_numbers
-from .window import attn_bwd_window, attn_fwd_window, mask_args
+from .window import attn_bwd_window, attn_fwd_window, mask_args, whole_number
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -42,7 +42,9 @@ def window_attention(q, k, v, window, sinks: int = 0, causal: bool = False, scal
     """attn_fwd_window with gradients for q, k and v."""
     window, sinks = mask_args(window, sinks)
     scale = None if scale is None else float(scale)
-    kw = dict(window=window, sinks=sinks, causal=causal, scale=scale, q_start=q_start, kv_lens=kv_lens)
+    if q_start is not None and not isinstance(q_start, torch.Tensor):
+        q_start = whole_number("q_start", q_start)
+    kw = dict(window=window, sinks=sinks, causal=bool(causal), scale=scale, q_start=q_start, kv_lens=kv_lens)
     return _WindowAttention.apply(q, k, v, kw)
 
 

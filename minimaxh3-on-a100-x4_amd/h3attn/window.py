@@ -23,7 +23,7 @@ from .ops import HEAD_DIM, _as_kernel_input, _layout, _on_device, _stream
 SPLIT_ROWS = 8192
 
 
-def _whole(name: str, n) -> int:
+def whole_number(name: str, n) -> int:
     """n as a plain int: read now, whatever may be written to it later."""
     try:
         return operator.index(n)
@@ -48,11 +48,11 @@ def mask_args(window, sinks):
     if type(left) is int and type(right) is int and type(sinks) is int:
         return (left, right), sinks
     if type(left) is not int and left is not None:
-        left = _whole("window's left side", left)
+        left = whole_number("window's left side", left)
     if type(right) is not int and right is not None:
-        right = _whole("window's right side", right)
+        right = whole_number("window's right side", right)
     if type(sinks) is not int and sinks is not None:
-        sinks = _whole("sinks", sinks)
+        sinks = whole_number("sinks", sinks)
     return (left, right), sinks
 
 
@@ -83,7 +83,7 @@ def _window(window, sinks, causal, q_start, kv_lens, B, Sq, Skv, device):
     if isinstance(q_start, torch.Tensor):
         starts, start = _per_sequence("q_start", q_start, B, device), None
     elif q_start is not None:
-        start = _whole("q_start", q_start)
+        start = whole_number("q_start", q_start)
     elif lens is not None and Sq != Skv:
         raise ValueError("kv_lens with Sq != Skv needs q_start: where the queries sit in the sequences")
     else:

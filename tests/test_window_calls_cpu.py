@@ -3,7 +3,11 @@ from __future__ import annotations
 
 import ctypes
 
-from h3attn import _lib, window
+import numpy as np
+import pytest
+import torch
+
+from h3attn import _lib, autograd, window
 
 S3 = _lib.strides3
 ROW = S3(0, 0, 128)
@@ -45,3 +49,18 @@ def test_workspace_size_knows_no_positions():
     assert L.h3a_attn_fwd_window(16, 16, 16, 16, None, 1, 2, 1, 140, 100, 128, *(ROW,) * 4, ctypes.byref(w), 0.1, None,
                                  0, None) == _lib.H3A_ERR_INVALID_ARG
     assert b"rows must lie at positions" in L.h3a_last_error()
+
+
+def test_the_backward_pass_sees_the_forwards_arguments(monkeypatch):
+    """A start or a flag that is written to between the passes (numpy scalars, 0-d arrays) is read once."""
+    calls = []
+    monkeypatch.setattr(autograd._WindowAttention, "apply", lambda q, k, v, kw: calls.append(kw))
+    start, causal = np.array(3), np.array(True)
+    autograd.window_attention(None, None, None, (4, 0), causal=causal, q_start=start)
+    start[...], causal[...] = 9, False
+    assert calls[0]["q_start"] == 3 and type(calls[0]["q_start"]) is int and calls[0]["causal"] is True
+    with pytest.raises(ValueError, match="q_start must be a whole number"):
+        autograd.window_attention(None, None, None, (4, 0), q_start=1.5)
+    lens = torch.zeros(2, dtype=torch.int32)
+    autograd.window_attention(None, None, None, (4, 0), q_start=lens, kv_lens=lens)
+    assert calls[1]["q_start"] is lens and calls[1]["causal"] is False
