@@ -19,7 +19,7 @@ constexpr float kStaleSumLimit = 0x1p16f;
 // a refresh: ps > kStaleSumLimit, +inf or NaN.  Compared as bit patterns, which
 // order like the values for ps >= +0 and put every NaN above the limit; a
 // float compare could be folded to "ps > limit", false for NaN, by a compiler
-// allowed to assume no NaNs (the library builds with -fno-honor-nans).  A
+// allowed to assume no NaNs (the dense kernels build with -fno-honor-nans).  A
 // negative ps, which no stage produces, also counts as a refresh.
 __host__ __device__ __forceinline__ bool stage_sum_needs_refresh(float ps) {
   return __builtin_bit_cast(uint32_t, ps) > __builtin_bit_cast(uint32_t, kStaleSumLimit);
