@@ -174,13 +174,32 @@ __device__ __forceinline__ void load_columns(u32x4 (&f)[8], const uint16_t *base
   clear_past(f, row, rows);
 }
 
+// The same products 32 rows at a time, in the compiler's order: scores of the rows of X, and
+// acc += Y^T F.
+template <class L>
+__device__ __forceinline__ f32x16 scores_32(const uint16_t *x, const u32x4 (&xf)[8], int k_rd) {
+  f32x16 s[1];
+  score_tile<L, 1>(x, xf, k_rd, s);
+  return s[0];
+}
+template <class L>
+__device__ __forceinline__ void product_32(f32x16 (&acc)[4], const uint16_t *y, const f32x16 &w, int t_rd) {
+  const f32x16 ws[1] = {w};
+  u32x4 f[2];
+  pack_p<1>(ws, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i & 3] = mfma_32x32x16(transposed_operand<L>(y, t_rd, i), f[i >> 2], acc[i & 3]);
+}
+__device__ __forceinline__ void clear(f32x16 (&acc)[4]) {
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{0.f};
+}
+
 // acc * mul, rounded to bf16, to rows row0 .. row0 + nrows - 1: through a wave-private
 // LDS tile, so that every store writes four whole rows.  Columns whose `live` is false
-// store zeros; patch(put) may replace rows: put(row, a, b) sets the lane's dims 2*lane and
-// 2*lane + 1.
-template <class Patch>
+// store zeros.
 __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul, bool live, uint8_t *tile,
-                                              uint16_t *base, int64_t stride, int nrows, int lane, Patch patch) {
+                                              uint16_t *base, int64_t stride, int nrows, int lane) {
   const int g = lane >> 5, l32 = lane & 31;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) {
@@ -193,9 +212,6 @@ __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul,
       *(u32x2 *)(tile + l32 * 256 + ((c ^ (l32 & 15)) << 4) + 8 * g) = val;
     }
   }
-  patch([&](int row, float x, float y) __attribute__((always_inline)) {
-    *(uint32_t *)(tile + row * 256 + (((lane >> 2) ^ (row & 15)) << 4) + 4 * (lane & 3)) = pack_bf16x2(x, y);
-  });
   const int ch = lane & 15;
   const __amdgpu_buffer_rsrc_t res = stage_rsrc(base, stride, nrows < 32 ? nrows : 32);
 #pragma unroll
@@ -207,54 +223,127 @@ __device__ __forceinline__ void store_columns(const f32x16 (&acc)[4], float mul,
 }
 
 // The kernels' products multiply a hidden pair's weight, 0, with what the hidden row holds,
-// which is not 0 where that is an infinity or NaN.  So a column whose sum is not finite is
-// taken again by its wave from the pairs that see each other alone: rare, and slow.
+// which is not 0 where that is an infinity or NaN.  So where a sum of a tile is not finite,
+// its stages are walked a second time: the values that are not finite are taken out of the
+// LDS tile that the product reads, once their places are noted, and every column is told
+// which of its sums a row that it sees makes infinite or NaN.  That is a second pass over the
+// same matrix products, whatever the values are and whoever sees them; its loops are simple
+// ones, one buffer and 32 rows at a time, so that they need no more registers than the first
+// pass's.  At H=16 S=4096, 511 keys to either side: forward 0.053 ms, with one bad row of V
+// 0.135 (each spoiled column summed again by itself: 6.0), with a bad channel of V 0.49 (6.4);
+// backward 0.20 ms, with one bad row of V 0.30 (8.8), with dO all infinite 0.81.
 
-// Columns (bit c: column c) of a wave's accumulators that hold a value that is not finite.
-__device__ __forceinline__ uint32_t spoiled_columns(const f32x16 (&acc)[4], bool counts) {
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// Whether one of the wave's sums that count is not finite (the same on all lanes).
+__device__ __forceinline__ bool spoiled(const f32x16 (&acc)[4], bool counts) {
   bool bad = false;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) bad |= (__float_as_uint(acc[dt][r]) & 0x7f800000u) == 0x7f800000u;
-  const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad && counts);
-  return (uint32_t)(lanes | lanes >> 32);
+    for (int r = 0; r < 16; ++r) bad |= !finite(acc[dt][r]);
+  return __builtin_amdgcn_ballot_w64(bad && counts) != 0;
 }
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// Whether a flag is set in one of a workgroup's four waves.
+__device__ __forceinline__ bool any_wave(bool flag, int (&flags)[4], int wave, int lane) {
+  if (lane == 0) flags[wave] = flag;
+  __syncthreads();
+  return (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+}
+
+// Where a stage's values are not finite: bit e of [row][c] is element 8*c + e; `up` for
+// +infinity, `down` for -infinity, both for NaN.
+template <int ROWS>
+struct BadValues {
+  __attribute__((aligned(16))) uint8_t up[ROWS][16], down[ROWS][16];
+};
+
+// Takes the values that are not finite out of a stage, and notes them: zeros in their
+// place, or (kWhole) in that of their whole row.  By NT threads.
+template <class L, bool kIsV, int ROWS, int NT, bool kWhole>
+__device__ __forceinline__ void take_out(uint16_t *tile, BadValues<ROWS> &bad, int thread) {
+#pragma unroll 1
+  for (int at = thread; at < ROWS * 16; at += NT) {
+    const int row = at >> 4, slot = at & 15, chunk = kIsV ? L::v_chunk(row, slot) : L::k_chunk(row, slot);
+    u32x4 x = *(const u32x4 *)(tile + 8 * at);
+    uint32_t up = 0, down = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t v = x[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+      if ((v & 0x7f80u) != 0x7f80u) continue;
+      if (v & 0x7fu || !(v & 0x8000u)) up |= 1u << e;
+      if (v & 0x7fu || v & 0x8000u) down |= 1u << e;
+      x[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+    }
+    bad.up[row][chunk] = (uint8_t)up;
+    bad.down[row][chunk] = (uint8_t)down;
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64((up | down) != 0);  // a row's 16 chunks: 16 lanes
+    if (kWhole && lanes >> (thread & 48) & 0xffffu) x = u32x4{0, 0, 0, 0};
+    if (lanes) *(u32x4 *)(tile + 8 * at) = x;
+  }
+}
+
+// The rows of a stage that hold such values, and 0 for the weights of those rows (32 of
+// them, in the accumulators' order).
+template <int ROWS>
+__device__ __forceinline__ uint64_t bad_rows(const BadValues<ROWS> &bad, int lane) {
+  const u32x4 any = *(const u32x4 *)bad.up[lane % ROWS] | *(const u32x4 *)bad.down[lane % ROWS];
+  return __builtin_amdgcn_ballot_w64(lane < ROWS && (any[0] | any[1] | any[2] | any[3]) != 0);
+}
+__device__ __forceinline__ void drop_rows(f32x16 &w, uint32_t rows, int g) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (rows >> (8 * (r >> 2) + 4 * g + (r & 3)) & 1) w[r] = 0.f;
+}
+
+// The sums of a lane's column that rows it sees make infinite or NaN: bit 16*dt + r is
+// acc[dt][r].  kSigns: the weights are probabilities, and an infinity keeps its sign; the
+// others' are 0 or NaN, and so NaN is what either makes.
+template <bool kSigns>
+struct BadSums {
+  uint64_t up = 0, down = 0;
+  // Bits 4*c .. 4*c + 3: the lane half's four bits of byte c.
+  __device__ __forceinline__ static uint64_t half_bits(u32x4 row, int g) {
+    uint64_t bits = 0;
+#pragma unroll
+    for (int k = 3; k >= 0; --k) {
+      uint32_t x = row[k] >> (4 * g) & 0x0f0f0f0fu;
+      x = (x | x >> 4) & 0x00ff00ffu;
+      bits = bits << 16 | ((x | x >> 8) & 0xffffu);
+    }
+    return bits;
+  }
+  // A stage's: sees(i), whether the lane's column sees row i, all(i), whether that makes all
+  // of its sums NaN (the row's weight being that).
+  template <int ROWS, class Sees, class All>
+  __device__ __forceinline__ void add(const BadValues<ROWS> &bad, int lane, Sees sees, All all) {
+    for (uint64_t rows = bad_rows(bad, lane); rows; rows &= rows - 1) {
+      const int i = __builtin_ctzll(rows);
+      const bool seen = sees(i);
+      if (__builtin_amdgcn_ballot_w64(seen && (kSigns ? up & down : up) != ~0ull) == 0) continue;
+      if (seen) {
+        const u32x4 u = *(const u32x4 *)bad.up[i], d = *(const u32x4 *)bad.down[i];
+        const uint64_t every = all(i) ? ~0ull : 0;
+        up |= half_bits(kSigns ? u : u | d, lane >> 5) | every;
+        if (kSigns) down |= half_bits(d, lane >> 5) | every;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(f32x16 (&acc)[4]) const {
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool u = up >> (16 * dt + r) & 1, d = kSigns ? down >> (16 * dt + r) & 1 : u;
+        if (u || d) acc[dt][r] += u && d ? __builtin_nanf("") : (u ? -kNegInf : kNegInf);
+      }
+  }
+};
 
 // Natural logarithm of l * 2^m: -inf for an empty sum, l where that is not finite.
 __device__ __forceinline__ float log_sum(float m, float l) {
   return !finite(l) ? l : (l > 0.f ? (m + log2f(l)) * kLn2 : kNegInf);
-}
-
-__device__ __forceinline__ float dot128(const uint16_t *x, const uint16_t *y) {
-  float sum = 0.f;
-  for (int d = 0; d < 128; d += 8) {
-    const u32x4 a = *(const u32x4 *)(x + d), b = *(const u32x4 *)(y + d);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum = fmaf(bf16_hi(a[i]), bf16_hi(b[i]), fmaf(bf16_lo(a[i]), bf16_lo(b[i]), sum));
-  }
-  return sum;
-}
-
-// acc (the lane's dims 2*lane, 2*lane + 1) += sum over rows row0 .. row0 + 63 below limit of
-// weight(row) * Y[row], over the rows for which sees(row).
-template <class Sees, class Weight>
-__device__ __forceinline__ void add_seen_rows(float2 &acc, int row0, int limit, const uint16_t *Y, int64_t stride, int lane,
-                                              Sees sees, Weight weight) {
-  const int row = row0 + lane;
-  const bool seen = row < limit && sees(row);
-  const float w = seen ? weight(row) : 0.f;
-  for (uint64_t left = __builtin_amdgcn_ballot_w64(seen); left; left &= left - 1) {
-    const int i = __builtin_ctzll(left);
-    const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
-    const uint32_t y = *(const uint32_t *)(Y + (int64_t)(row0 + i) * stride + 2 * lane);
-    acc.x = fmaf(wi, bf16_lo(y), acc.x);
-    acc.y = fmaf(wi, bf16_hi(y), acc.y);
-  }
-}
-__device__ __forceinline__ float lane_value(float x, int lane) {
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
 // DMA of the rows of [row0, limit) that a tile holds, the rest as zeros.
@@ -360,20 +449,6 @@ __device__ __forceinline__ Item item_of(const WindowArgs &a, int i, int chunk, i
   return {bh < a.B * heads && tile < tiles ? tile : -1, bh % heads, bh / heads};
 }
 
-// add_seen_rows over all keys that position pos sees: weights weight(key, its row of K),
-// rows of Y.
-template <class Weight>
-__device__ __forceinline__ void each_seen_key(const WindowArgs &a, const Span &sp, int pos, const uint16_t *K,
-                                              const uint16_t *Y, int64_t ystride, int lane, float2 &sum,
-                                              Weight weight) {
-  KeyStages<> st;
-  st.init(a, sp, pos, pos);
-  for (int j = 0; j < st.n; ++j)
-    add_seen_rows(
-        sum, st.key0(j), st.limit(j), Y, ystride, lane, [](int) { return true; },
-        [&](int key) { return weight(key, K + (int64_t)key * a.kss); });
-}
-
 // Forward.  A workgroup takes 128 query rows of one head, a wave 32 of them; the
 // 64-key stages of their window are double-buffered in LDS by DMA, two workgroups to a
 // CU, so that one's softmax overlaps the other's MFMAs.  The softmax runs against a stale
@@ -385,6 +460,8 @@ __device__ __forceinline__ void each_seen_key(const WindowArgs &a, const Span &s
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_fwd_kernel(WindowArgs a) {
   using L = SwzLayout;
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][StageBytes<L>::kK / 2], vbuf[2][StageBytes<L>::kV / 2];
+  __shared__ BadValues<kBN> bad;
+  __shared__ int flags[4];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item it = item_of(a, (int)blockIdx.x, a.chunk, a.nqt, a.H);
@@ -436,6 +513,33 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       wait_vmem_all();
       __syncthreads();
     });
+    // (A column whose own scores are not finite is NaN throughout, whatever V holds.)
+    if (any_wave(spoiled(o, live && finite(half_swap_sum(lsum))), flags, wave, lane)) {
+      BadSums<true> seen;
+      clear(o);
+      m = kNegInf, lsum = 0.f;
+      for (int j = 0; j < st.n; ++j) {
+        fetch(j, C<0>{});
+        wait_vmem_all();
+        __syncthreads();
+        take_out<L, true, kBN, 256, false>(vbuf[0], bad, tid);
+        __syncthreads();
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          f32x16 s[1] = {scores_32<L>(kbuf[0] + u * 32 * 128, qf, k_rd)};
+          u32x4 pf[2];
+          mask_band(s, st.key0(j) + 32 * u, g, lo, hi, first, j < st.n_first, kNegInf);
+          softmax_stage<1>(s, 0, 32, g, a.sl2, m, lsum, o, pf);
+          pv_tile<L, 2>(vbuf[0] + u * 32 * 128, pf, v_rd, o);
+        }
+        seen.add(bad, lane, [&](int i) {
+          const int key = st.key0(j) + i;
+          return (j >= st.n_first && key >= lo && key <= hi) || key < first;
+        }, [](int) { return false; });
+        __syncthreads();
+      }
+      seen.put(o);
+    }
   }
   const float ltot = half_swap_sum(lsum);
   const float inv = ltot > 0.f ? 1.f / ltot : 0.f;
@@ -443,19 +547,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     a.lse[((int64_t)it.b * a.H + it.h) * a.Sq + row] = live ? log_sum(m, ltot) : kNegInf;
   if (wq0 < a.Sq)
     store_columns(o, inv, live, reinterpret_cast<uint8_t *>(&kbuf[0][0]) + wave * 8192,
-                  a.o + it.b * a.osb + it.h * a.osh + (int64_t)wq0 * a.oss, a.oss, a.Sq - wq0, lane,
-                  [&](auto put) __attribute__((always_inline)) {
-                    for (uint32_t left = spoiled_columns(o, live && finite(ltot)); left; left &= left - 1) {
-                      const int c = __builtin_ctz(left), r = wq0 + c;
-                      const float mc = lane_value(m, c), ic = lane_value(inv, c);
-                      const uint16_t *q = a.q + it.b * a.qsb + it.h * a.qsh + (int64_t)r * a.qss;
-                      float2 sum = {0.f, 0.f};
-                      each_seen_key(a, sp, sp.qs + r, Kb, Vb, a.vss, lane, sum, [&](int, const uint16_t *k) {
-                        return fast_exp2(fmaf(dot128(q, k), a.sl2, -mc));
-                      });
-                      put(c, sum.x * ic, sum.y * ic);
-                    }
-                  });
+                  a.o + it.b * a.osb + it.h * a.osh + (int64_t)wq0 * a.oss, a.oss, a.Sq - wq0, lane);
 }
 
 // Forward for few query rows (a new token, or a short chunk of them, against a cache).
@@ -467,6 +559,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 constexpr int kTokenStage = 32, kTokenRows = 32;
 struct TokenLds {
   uint16_t k[4][2][kTokenStage * 128], v[4][2][kTokenStage * 128];  // by wave
+  BadValues<kTokenStage> bad[4];
 };
 
 // Column c of a key head's group of 32 -> query row and head among those that share it
@@ -546,6 +639,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
       softmax_stage<1>(s, 0, kTokenStage, g, a.sl2, m, lsum, o, pf);
       pv_tile<L, 2>(lds.v[wave][buf], pf, v_rd, o);
     }
+    if (spoiled(o, live && finite(half_swap_sum(lsum)))) {
+      BadSums<true> seen;
+      clear(o);
+      m = kNegInf, lsum = 0.f;
+      for (j = j_a + wave; j < j_b; j += 4) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fetch(j, 0);
+        wait_vmem_all();
+        asm volatile("" ::: "memory");
+        take_out<L, true, kTokenStage, 64, false>(lds.v[wave][0], lds.bad[wave], lane);
+        f32x16 s[1] = {scores_32<L>(lds.k[wave][0], qf, k_rd)};
+        u32x4 pf[2];
+        mask_band(s, st.key0(j), g, lo, hi, first, j < st.n_first, kNegInf);
+        softmax_stage<1>(s, 0, kTokenStage, g, a.sl2, m, lsum, o, pf);
+        pv_tile<L, 2>(lds.v[wave][0], pf, v_rd, o);
+        seen.add(lds.bad[wave], lane, [&](int i) {
+          const int key = st.key0(j) + i;
+          return (j >= st.n_first && key >= lo && key <= hi) || key < first;
+        }, [](int) { return false; });
+      }
+      seen.put(o);
+    }
   }
   // Merge the waves: wave u takes dims 32u .. 32u+31 of all four.
   __syncthreads();
@@ -556,33 +671,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) xch[((wave * 4 + dt) * 16 + r) * 64 + lane] = o[dt][r];
-  for (uint32_t left = spoiled_columns(o, live && finite(ltot)); left; left &= left - 1) {
-    const int c = __builtin_ctz(left);
-    const TokenColumn tc = token_column(a, group, c);
-    const int hc = hk * a.rep + tc.head, pc = sp.qs + tc.row;
-    const float mc = lane_value(m, c);
-    const uint16_t *q = a.q + b * a.qsb + hc * a.qsh + (int64_t)tc.row * a.qss;
-    const int lo = pc - a.left, first = first_keys(a, sp, pc);
-    const int hi = pc + a.right < sp.len - 1 ? pc + a.right : sp.len - 1;
-    KeyStages<kTokenStage> st;
-    st.init(a, sp, sp.qs + r0, sp.qs + r1);
-    const int j_a = (int)((int64_t)st.n * piece / a.pieces), j_b = (int)((int64_t)st.n * (piece + 1) / a.pieces);
-    float2 sum = {0.f, 0.f};
-    for (int j = j_a + wave; j < j_b; j += 4) {
-      const int end = st.key0(j) + kTokenStage;
-      add_seen_rows(
-          sum, st.key0(j), end < st.limit(j) ? end : st.limit(j), a.v + b * a.vsb + hk * a.vsh, a.vss, lane,
-          [&](int key) { return (j >= st.n_first && key >= lo && key <= hi) || key < first; },
-          [&](int key) {
-            return fast_exp2(fmaf(dot128(q, a.k + b * a.ksb + hk * a.ksh + (int64_t)key * a.kss), a.sl2, -mc));
-          });
-    }
-    // Dims 2*lane and 2*lane + 1 of column c in the accumulators' order.
-    const int d = 2 * lane, r = 4 * ((d & 31) >> 3) + (d & 3);
-    float *at = xch + ((wave * 4 + (d >> 5)) * 16 + r) * 64 + 32 * ((d >> 2) & 1) + c;
-    at[0] = sum.x;
-    at[64] = sum.y;
-  }
   ml[wave * 64 + lane] = float2{m, ltot};
   __syncthreads();
   float top = kNegInf, l = 0.f, w[4];
@@ -700,6 +788,8 @@ __device__ __forceinline__ bool few_keys(const WindowArgs &a, const Span &s, int
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) window_dq_kernel(WindowArgs a) {
   using L = DualLayout;
   __shared__ __attribute__((aligned(16))) uint16_t kbuf[2][StageBytes<L>::kK / 2], vbuf[2][StageBytes<L>::kK / 2];
+  __shared__ BadValues<kBN> bad;
+  __shared__ int flags[4];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item it = item_of(a, (int)blockIdx.x, a.chunk, a.nqt, a.H);
@@ -804,23 +894,47 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       wait_vmem_all();
       __syncthreads();
     });
+    // (A row whose own statistics are not finite is NaN throughout.)  Rows of K that are not
+    // finite are taken out whole, with weight 0: K is also what the scores are from, and in a
+    // row whose lse is finite the score of such a key is -inf.
+    const bool own = !finite(delta) || l2 != l2;
+    if (any_wave(spoiled(dq, live && !own), flags, wave, lane)) {
+      BadSums<false> seen;
+      clear(dq);
+      for (int j = 0; j < st.n; ++j) {
+        fetch(j, C<0>{});
+        wait_vmem_all();
+        __syncthreads();
+        take_out<L, false, kBN, 256, true>(kbuf[0], bad, tid);
+        __syncthreads();
+        const uint64_t out = bad_rows(bad, lane);
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          f32x16 s = scores_32<L>(kbuf[0] + u * 32 * 128, qf, k_rd);
+          const f32x16 dp = scores_32<L>(vbuf[0] + u * 32 * 128, df, k_rd);
+          const int key0 = st.key0(j) + 32 * u + 4 * g, low = j < st.n_first ? 1 << 30 : lo;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = key0 + 8 * (r >> 2) + (r & 3);
+            s[r] = fast_exp2(fmaf(s[r], a.sl2, -l2)) * (dp[r] - delta);
+            if (!((at >= low && at <= hi) || at < first)) s[r] = 0.f;
+          }
+          drop_rows(s, (uint32_t)(out >> 32 * u), g);
+          product_32<L>(dq, kbuf[0] + u * 32 * 128, s, t_rd);
+        }
+        seen.add(bad, lane, [&](int i) {
+          const int key = st.key0(j) + i;
+          return (j >= st.n_first && key >= lo && key <= hi) || key < first;
+        }, [](int) { return false; });
+        __syncthreads();
+      }
+      if (own) seen.up = ~0ull;
+      seen.put(dq);
+    }
   }
   if (wq0 < a.Sq)
     store_columns(dq, a.scale, live, reinterpret_cast<uint8_t *>(&kbuf[0][0]) + wave * 8192,
-                  a.dq + it.b * a.dqsb + it.h * a.dqsh + (int64_t)wq0 * a.dqss, a.dqss, a.Sq - wq0, lane,
-                  [&](auto put) __attribute__((always_inline)) {
-                    for (uint32_t left = spoiled_columns(dq, live && finite(delta)); left; left &= left - 1) {
-                      const int c = __builtin_ctz(left), r = wq0 + c;
-                      const float lc = lane_value(l2, c), dc = lane_value(delta, c);
-                      const uint16_t *q = a.q + it.b * a.qsb + it.h * a.qsh + (int64_t)r * a.qss;
-                      const uint16_t *d = a.dout + it.b * a.gsb + it.h * a.gsh + (int64_t)r * a.gss;
-                      float2 sum = {0.f, 0.f};
-                      each_seen_key(a, sp, sp.qs + r, Kb, Kb, a.kss, lane, sum, [&](int key, const uint16_t *k) {
-                        return fast_exp2(fmaf(dot128(q, k), a.sl2, -lc)) * (dot128(d, Vb + (int64_t)key * a.vss) - dc);
-                      });
-                      put(c, sum.x * a.scale, sum.y * a.scale);
-                    }
-                  });
+                  a.dq + it.b * a.dqsb + it.h * a.dqsh + (int64_t)wq0 * a.dqss, a.dqss, a.Sq - wq0, lane);
 }
 
 // Backward, dK and dV: a workgroup sums one of them over 128 keys of one key head, a wave
@@ -846,6 +960,8 @@ constexpr int kQStage = 64;
 struct DkdvLds {
   uint16_t q[2][kQStage * 128], dout[2][kQStage * 128];
   float stats[2][2][kQStage];  // lse (log2 units), delta
+  BadValues<kQStage> bad;
+  int flags[4];
 };
 
 // Where a piece's dK (which 0) or dV of 128 keys by 128 dims is in a.part: those of the first
@@ -986,58 +1102,60 @@ __device__ __forceinline__ void window_key_sums(const WindowArgs &a, const Item 
       wait_vmem_all();
       __syncthreads();
     });
+    // For dK, rows of Q that are not finite are taken out whole, with weight 0 (as keys are in
+    // window_dq_kernel): such a row's lse is NaN, and with it every sum of a key that it sees,
+    // or -inf, and its weights are 0.
+    if (any_wave(spoiled(acc, key < sp.len), lds.flags, wave, lane)) {
+      BadSums<!kDk> seen;
+      clear(acc);
+      fh = it.h * a.rep + (int)(t_a / per_head), frow = i_a + (int)(t_a % per_head) * kQStage;
+      for (int j = 0; j < n; ++j) {
+        const int p0 = sp.qs + frow, rows = i_b - frow;
+        fetch(C<0>{});
+        wait_vmem_all();
+        __syncthreads();
+        take_out<L, false, kQStage, 256, kDk>(kDk ? lds.q[0] : lds.dout[0], lds.bad, tid);
+        __syncthreads();
+        const uint64_t out = kDk ? bad_rows(lds.bad, lane) : 0;
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          f32x16 s = scores_32<L>(lds.q[0] + u * 32 * 128, kf, k_rd), dp = {0.f};
+          if constexpr (kDk) dp = scores_32<L>(lds.dout[0] + u * 32 * 128, vf, k_rd);
+          const uint32_t ahead = (uint32_t)(p0 + 32 * u + 4 * g - plo);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = 32 * u + 8 * (r >> 2) + 4 * g + (r & 3);
+            const float p = fast_exp2(fmaf(s[r], a.sl2, -lds.stats[0][0][at]));
+            s[r] = kDk ? p * (dp[r] - lds.stats[0][1][at]) : p;
+            // (Rows past i_b are zeros, but 0 times an infinity of the key's is not.)
+            if (ahead + 8 * (r >> 2) + (r & 3) > span || at >= rows) s[r] = 0.f;
+          }
+          if (kDk) drop_rows(s, (uint32_t)(out >> 32 * u), g);
+          product_32<L>(acc, (kDk ? lds.q[0] : lds.dout[0]) + u * 32 * 128, s, t_rd);
+        }
+        seen.add(lds.bad, lane, [&](int i) { return (uint32_t)(p0 + i - plo) <= span; }, [&](int i) {
+          const float l2 = lds.stats[0][0][i];
+          return kDk && (l2 != l2 || !finite(lds.stats[0][1][i]));
+        });
+        __syncthreads();
+      }
+      seen.put(acc);
+    }
   }
-  // Column c of this piece again, from the rows that see it.
-  auto column_again = [&](int c) __attribute__((always_inline)) -> float2 {
-    float2 sum = {0.f, 0.f};
-    const int key_c = wj0 + c, plo_c = key_c < a.sinks ? (a.causal ? key_c : -(1 << 30)) : key_c - a.right;
-    const uint32_t span_c = key_c < a.sinks ? 0x7fffffffu : (uint32_t)(a.left + a.right);
-    const uint16_t *k = a.k + it.b * a.ksb + it.h * a.ksh + (int64_t)key_c * a.kss;
-    const uint16_t *v = a.v + it.b * a.vsb + it.h * a.vsh + (int64_t)key_c * a.vss;
-    for (int64_t t = t_a; t < t_a + n; ++t) {
-      const int h = it.h * a.rep + (int)(t / per_head), row0 = i_a + (int)(t % per_head) * kQStage;
-      const uint16_t *q = a.q + it.b * a.qsb + h * a.qsh, *d = a.dout + it.b * a.gsb + h * a.gsh;
-      const float *st = a.stats + ((int64_t)it.b * a.H + h) * a.Sq;
-      add_seen_rows(
-          sum, row0, i_b, kDk ? q : d, kDk ? a.qss : a.gss, lane,
-          [&](int row) { return (uint32_t)(sp.qs + row - plo_c) <= span_c; },
-          [&](int row) {
-            const float p = fast_exp2(fmaf(dot128(q + (int64_t)row * a.qss, k), a.sl2, -st[row]));
-            return kDk ? p * (dot128(d + (int64_t)row * a.gss, v) - st[a.stats_n + row]) : p;
-          });
-    }
-    return sum;
-  };
-  const uint32_t spoiled = n > 0 ? spoiled_columns(acc, key < sp.len) : 0;
   if (pieces > 1) {
-    float *part = a.part + part_slot(a, it.b * a.Hkv + it.h, it.tile, piece, kDk ? 0 : 1) + 32 * wave * 128;
-    if (!(spoiled >> l32 & 1)) {
-      float *p = part + l32 * 128 + 4 * g;
+    float *p = a.part + part_slot(a, it.b * a.Hkv + it.h, it.tile, piece, kDk ? 0 : 1) + (32 * wave + l32) * 128 + 4 * g;
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
+    for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-        for (int rr = 0; rr < 4; ++rr)
-          *(float4 *)(p + dt * 32 + 8 * rr) =
-              key < sp.len ? float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]}
-                           : float4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (uint32_t left = spoiled; left; left &= left - 1) {
-      const int c = __builtin_ctz(left);
-      *(float2 *)(part + c * 128 + 2 * lane) = column_again(c);
-    }
+      for (int rr = 0; rr < 4; ++rr)
+        *(float4 *)(p + dt * 32 + 8 * rr) =
+            key < sp.len ? float4{acc[dt][4 * rr], acc[dt][4 * rr + 1], acc[dt][4 * rr + 2], acc[dt][4 * rr + 3]}
+                         : float4{0.f, 0.f, 0.f, 0.f};
   } else if (wj0 < a.Skv) {
     uint8_t *tile = reinterpret_cast<uint8_t *>(&lds.q[0][0]) + wave * 8192;
     uint16_t *out = kDk ? a.dk + it.b * a.dksb + it.h * a.dksh + (int64_t)wj0 * a.dkss
                         : a.dv + it.b * a.dvsb + it.h * a.dvsh + (int64_t)wj0 * a.dvss;
-    const float mul = kDk ? a.scale : 1.f;
-    store_columns(acc, mul, key < sp.len, tile, out, kDk ? a.dkss : a.dvss, a.Skv - wj0, lane,
-                  [&](auto put) __attribute__((always_inline)) {
-                    for (uint32_t left = spoiled; left; left &= left - 1) {
-                      const int c = __builtin_ctz(left);
-                      const float2 sum = column_again(c);
-                      put(c, sum.x * mul, sum.y * mul);
-                    }
-                  });
+    store_columns(acc, kDk ? a.scale : 1.f, key < sp.len, tile, out, kDk ? a.dkss : a.dvss, a.Skv - wj0, lane);
   }
 }
 

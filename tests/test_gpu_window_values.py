@@ -77,6 +77,54 @@ def test_bad_values_reach_who_sees_them(gpu, B, H, Hkv, S, window, sinks, bad, w
     assert spread  # the bad values are seen by someone
 
 
+@pytest.mark.parametrize("B,H,Hkv,S,window,sinks", SHAPES)
+def test_a_key_that_no_row_takes(gpu, B, H, Hkv, S, window, sinks):
+    """A key whose scores are all -inf has weight 0: O, dk and dv are as without it, dq is NaN where 0 meets its infinity."""
+    q, k, v, do = make(gpu, B, H, Hkv, S, S, 9)
+    q[..., 11] = -q[..., 11].abs() - 0.125
+    spots = (sinks + 1, S // 2, S - 1)
+    for at in spots:
+        k[:, :, at, 11] = float("inf")
+    mask = ref.visible(B, S, S, window, sinks, False, None, None)
+    kw = dict(window=window, sinks=sinks)
+    o, lse = h3attn.attn_fwd_window(q, k, v, return_lse=True, **kw)
+    dq, dk, dv = h3attn.attn_bwd_window(do, q, k, v, o, lse, **kw)
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all() and torch.isfinite(dk).all() and torch.isfinite(dv).all()
+    assert (dk[:, :, spots] == 0).all() and (dv[:, :, spots] == 0).all()
+    rep = H // Hkv
+    for b, hk in {(0, 0), (B - 1, Hkv - 1)}:
+        kv_out, kv_bound = [0, 0], [0, 0]
+        for h in range(hk * rep, (hk + 1) * rep):
+            outs, bounds = by_definition(*(t.cpu() for t in (q[b, h], k[b, hk], v[b, hk], do[b, h])), mask[b])
+            assert torch.isnan(outs[1]).any()
+            kv_out = [x + y for x, y in zip(kv_out, outs[2:])]
+            kv_bound = [x + y for x, y in zip(kv_bound, bounds[2:])]
+            compare("O", o[b, h], outs[0], bounds[0])
+            compare("dq", dq[b, h], outs[1], bounds[1])
+        compare("dk", dk[b, hk], kv_out[0], kv_bound[0])
+        compare("dv", dv[b, hk], kv_out[1], kv_bound[1])
+
+
+@pytest.mark.parametrize("S", [200, 700])
+def test_infinities_keep_their_sign(gpu, S):
+    """A weight is never negative: +inf in v, or in dout, is +inf in O, or dv, and NaN only where -inf meets it."""
+    q, k, v, do = make(gpu, 1, 2, 2, S, S, 5)
+    inf, at = float("inf"), S // 2
+    for t in (v, do):
+        t[:, :, at, 3], t[:, :, at, 4], t[:, :, at, 5] = inf, -inf, inf
+        t[:, :, at + 1, 5] = -inf
+        t[:, :, at + 30, 6] = inf  # hidden from half of those that see the others
+    o, lse = h3attn.attn_fwd_window(q, k, v, (20, 20), return_lse=True)
+    near = slice(at - 8, at + 9)
+    far = torch.ones(S, dtype=torch.bool)
+    far[at - 20:at + 51] = False
+    for name, t in (("O", o), ("dv", h3attn.attn_bwd_window(do, q, k, k, o := h3attn.attn_fwd_window(q, k, k, (20, 20)),
+                                                             lse, (20, 20))[2])):
+        assert (t[:, :, near, 3] == inf).all() and (t[:, :, near, 4] == -inf).all(), name
+        assert torch.isnan(t[:, :, near, 5]).all() and torch.isfinite(t[:, :, near, 6]).all(), name
+        assert torch.isfinite(t[:, :, near, 7:]).all() and torch.isfinite(t[:, :, far.to(t.device)]).all(), name
+
+
 def compare(name, got, want, bound):
     got = got.cpu().double()
     fine = torch.isfinite(want)
@@ -86,3 +134,57 @@ def compare(name, got, want, bound):
     limit = (bound + (BF16 + FP32) * want.abs() + 1e-30)[fine]
     assert (err <= limit).all(), f"{name}: error {(err / limit).max():.3f} of what the roundings allow"
     return (~fine).sum().item()
+
+
+def pass_time(fn):
+    """Milliseconds of a call, the better of two."""
+    fn()
+    times = []
+    for _ in range(2):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        fn()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+# As many heads as fill the chip with tiles, one whose keys are split, and rows of one token each.
+@pytest.mark.parametrize("B,H,Hkv,Sq,S", [(1, 16, 16, 4096, 4096), (1, 1, 1, 2048, 2048), (16, 28, 4, 1, 4096)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("what,where", [("do", "all"), ("do", "row"), ("do", "element"), ("do", "last"), ("q", "all"),
+                                        ("q", "row"), ("q", "element"), ("k", "all"), ("k", "row"), ("k", "element"),
+                                        ("v", "all"), ("v", "row"), ("v", "element"), ("v", "channel")])
+def test_bad_values_that_are_seen_cost_little(gpu, B, H, Hkv, Sq, S, bad, what, where):
+    """A step whose gradient overflowed, or one bad token, takes some times a clean one's time, not hundreds.
+
+    A tile with a sum that is not finite is walked once more, in simpler loops (two to three times
+    as long) that note every bad row (a few times as long again if each row is one).
+    """
+    t = dict(zip("q k v do".split(), make(gpu, B, H, Hkv, Sq, S, 3)))
+    kw = dict(window=(511, 0 if Sq == 1 else 511), sinks=40)
+    kw.update(q_start=torch.full((B,), S - 1, dtype=torch.int32, device=gpu) if Sq == 1 else None)
+
+    def fwd():
+        return h3attn.attn_fwd_window(t["q"], t["k"], t["v"], return_lse=True, **kw)
+
+    def bwd():
+        return h3attn.attn_bwd_window(t["do"], t["q"], t["k"], t["v"], *out, **kw)
+
+    out = fwd()
+    clean = [pass_time(fwd), pass_time(bwd)]
+    n = t[what].shape[2]
+    mid = n - 1 if where == "last" or n > Sq else n // 2
+    if where == "all":
+        t[what].fill_(bad)
+    elif where == "channel":
+        t[what][..., 77] = bad
+    elif where == "element":
+        t[what][:, :, mid, 77] = bad
+    else:
+        t[what][:, :, mid] = bad
+    out = fwd()
+    spoiled = [pass_time(fwd), pass_time(bwd)]
+    print(f"{what} {where} {bad}: forward {clean[0]:.3f} -> {spoiled[0]:.3f} ms, backward {clean[1]:.3f} -> {spoiled[1]:.3f}")
+    assert spoiled[0] <= 16 * clean[0] + 0.05 and spoiled[1] <= 16 * clean[1] + 0.05
