@@ -164,10 +164,11 @@ def attn_fwd_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, s
 
 
 def _rows_apart(name: str, t: torch.Tensor):
-    """t and its strides with rows that do not overlap, copied where they do (a gradient expanded over the sequence)."""
+    """t and its strides with rows that do not overlap and lie on the 16-byte grid, copied where they do not: a
+    gradient may be expanded over the sequence (that of a mean) or a piece of a larger one (that of a concatenation)."""
     t, st = _as_kernel_input(name, t)
-    if t.shape[2] > 1 and st[2] < HEAD_DIM:
-        t, st = _as_kernel_input(name, t.contiguous())
+    if (t.shape[2] > 1 and st[2] < HEAD_DIM) or t.data_ptr() & 15:
+        t, st = _as_kernel_input(name, t.clone(memory_format=torch.contiguous_format))
     return t, st
 
 

@@ -50,3 +50,17 @@ def test_more_rows_than_keys(gpu, B, H, Hkv, Sq, Skv, causal):
     check(gpu, B, H, Hkv, Sq, Skv, (40, 0 if causal else 25), 6, causal, q_start=starts)
     check(gpu, B, H, Hkv, Sq, Skv, (40, 0 if causal else 25), 6, causal, q_start=starts,
           kv_lens=[Skv - 1, Skv // 2, Skv, 0][:B])
+
+
+@pytest.mark.parametrize("offset", [1, 3, 4, 8])
+def test_gradient_off_the_16_byte_grid(gpu, offset):
+    """The gradient of an output that was concatenated behind an odd number of other values is a piece of a larger one."""
+    B, H, S = 1, 2, 70
+    q, k, v, do = make(gpu, B, H, H, S, S, seed=2)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = autograd.window_attention(*leaves, (12, 12))
+    both = torch.cat([torch.zeros(offset, dtype=torch.bfloat16, device=gpu), o.reshape(-1)])
+    both.backward(torch.cat([torch.zeros(offset, dtype=torch.bfloat16, device=gpu), do.reshape(-1)]))
+    o2, lse = h3attn.attn_fwd_window(q, k, v, (12, 12), return_lse=True)
+    for t, want in zip(leaves, h3attn.attn_bwd_window(do, q, k, v, o2, lse, (12, 12))):
+        assert torch.equal(t.grad, want)
