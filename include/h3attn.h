@@ -401,8 +401,8 @@ int h3a_qk_rmsnorm_rope_pool(void *q, void *k, int B, int S, int H, int D,
  * axis, hold i; as pair n of an axis of d dims it turns by
  *   angle = pos[b,s,axis] * theta^(-2n/d)
  * in the sense of h3a_qk_rmsnorm_rope's R = [[cos, -sin], [sin, cos]].  Angles are
- * taken in 64 bits.  dims: even; rot a multiple of 16, <= D.  No counterpart in the
- * reference, whose caller brings the table.
+ * taken in 64 bits.  dims: even; rot a multiple of 16, <= D.  qw, kw: bf16 [D], as
+ * there.  No counterpart in the reference, whose caller brings the table.
  */
 #define H3A_MAX_AXES 4
 typedef struct {

@@ -68,7 +68,12 @@ class _QkNormRope(torch.autograd.Function):
 
 
 def qk_norm_rope(q, k, pos, axes, qw, kw, eps: float = 1e-6, theta: float = 10000.0):
-    """qk_rmsnorm_rope_axes (out of place) with gradients for q, k and the weights, those in the weights' dtype."""
+    """qk_rmsnorm_rope_axes (out of place) with gradients for q, k and the weights, those in the weights' dtype.
+
+    Weights kept in fp32 take part rounded to bf16, in both passes: their gradients are
+    not rounded, but an update of less than half a bf16 step (2^-8 of the weight) shows in
+    the output only once such updates have added up to it.
+    """
     return _QkNormRope.apply(q, k, pos, qw, kw, whole_numbers("axes", axes), float(eps), float(theta))
 
 

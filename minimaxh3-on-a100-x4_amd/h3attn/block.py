@@ -52,6 +52,7 @@ def _rope_output(name: str, t, shape, device):
 
 
 def _rope_weight(name: str, w: torch.Tensor, device) -> torch.Tensor:
+    """The weights as the kernels read them: bf16, as in qk_rmsnorm_rope_ (a model's are; others are rounded)."""
     if w.numel() != HEAD_DIM:
         raise ValueError(f"{name} must have {HEAD_DIM} elements")
     if w.dtype != torch.bfloat16 or w.device != device or not w.is_contiguous() or w.data_ptr() & 15:
@@ -103,6 +104,7 @@ def qk_rmsnorm_rope_axes(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, ax
     rot is a multiple of 16; pair (i, i + rot/2) belongs to the axis whose dims/2
     pairs hold i, and as its n-th pair turns by pos * theta^(-2n/dims).  With one
     axis these are the rotations of rope_freqs.  Dims from rot on are only normalised.
+    qw, kw: 128 weights, used in bf16: those of another dtype are rounded to it first.
     out: (q', k') to write, for instance (q, k) themselves.
     """
     (q, k, pos, qw, kw), p, sizes, (qst, kst) = _rope_prepare(q, k, pos, axes, qw, kw, theta)
@@ -130,7 +132,7 @@ def qk_rmsnorm_rope_axes_bwd(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor
     """Gradients of qk_rmsnorm_rope_axes from those of its outputs: (q's, k's, qw's, kw's).
 
     q and k are the forward's inputs.  The weights' gradients are fp32 [128], summed
-    over all rows in a fixed order.
+    over all rows in a fixed order, at the weights as the forward uses them (in bf16).
     """
     (q, k, pos, qw, kw), p, (B, S, Hq, Hk, D), (qst, kst) = _rope_prepare(q, k, pos, axes, qw, kw, theta)
     if dq.shape != q.shape or dk.shape != k.shape:
