@@ -176,7 +176,6 @@ int norm_wgs(const int *bounds, int segments, int rows_per_wg);
 int launch_layer_norm(NormArgs a, const int *bounds, int segments, int dtype, bool bwd, bool vec, hipStream_t s);
 
 // Argument block of the prologue from positions (h3a_prologue.hip).
-constexpr int kRopeAxes = 4;
 struct RopeAxesArgs {
   const uint16_t *x[2];   // q, k [B,S,H,128]: strides {batch, seq, head}
   const uint16_t *dy[2];  // backward: gradients of the outputs

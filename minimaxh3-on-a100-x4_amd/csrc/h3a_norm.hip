@@ -8,7 +8,8 @@
 // Bound by HBM: every row is read once and written once.  A row is held in registers by
 // one wave (short rows) or one workgroup, 8 consecutive channels per thread and step;
 // a workgroup walks consecutive rows of one segment, so that the segment's weights, and
-// in the backward pass the sums of dw and db, stay in registers.  Those sums leave as
+// in the backward pass the sums of dw and db, stay in registers (past 8192 channels the
+// backward pass keeps 50 to 249 of them in scratch memory).  Those sums leave as
 // one fp32 partial row per workgroup and are added by a second kernel in a fixed order.
 // Statistics and sums are fp32; the variance is taken about the row's own mean.
 #include "h3a_device.h"
@@ -395,8 +396,12 @@ NormKernel pick(int dtype, int C, int *rows_at_once) {
 }  // namespace
 
 // Rows per workgroup, in whole steps of the rows it takes at once: as many as make the
-// workgroups just fit the chip's 256 CUs at once, each segment adding at most one (13
-// more than fit took 408 us for 335 at 42120 rows of 5376 channels, backward).
+// grid per_cu workgroups on each of the chip's 256 CUs, each segment adding at most one (13
+// more than fit took 408 us for 335 at 42120 rows of 5376 channels, backward).  per_cu is by
+// width alone, and what fits goes by type and alignment too: backward, one workgroup fewer
+// fits from 1025 to 2048 and from 6145 channels on, and up to 512 in fp32 and at odd widths
+// of bf16, forward half as many past 8192; these run the rest of the grid as a second round
+// (bf16 backward: 3.9 TB/s at 2048 and 8192 channels, 4.2 to 4.8 at 512, 1024, 4096 and 5376).
 int norm_rows_per_wg(int64_t rows, int C, int segments, bool bwd) {
   const int per_cu = bwd ? (C <= 512 || (C > 1024 && C <= 2048) ? 5 : (C <= 1024 ? 3 : 2)) : (C <= 2048 ? 8 : 4);
   const int wgs = 256 * per_cu - (segments < 128 ? segments : 0);

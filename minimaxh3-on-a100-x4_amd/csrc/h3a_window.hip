@@ -777,7 +777,7 @@ __device__ __forceinline__ bool few_keys(const WindowArgs &a, const Span &s, int
 
 // Backward, dQ: tiles and stages as forward, with P from the stored lse.  The rows' lse
 // (log2 units; +inf, so that p = 0, for a row that saw nothing) and delta = dO.O go to
-// a.stats for the second kernel.  O's rounding to bf16 makes delta off by 2^-9 of what the
+// a.stats for the second kernel.  O's rounding to bf16 makes delta off by up to 2^-8 of what the
 // few keys of a row near a sequence's start or under a narrow window give, which there is
 // as much as dS itself (a row of one key has dS = 0): such tiles take sum p dP in a pass of
 // their own instead (relative error of dQ and dK, S=100 causal: 0.0029 -> 0.0024, which is
@@ -947,7 +947,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // waves per SIMD wait for every operand and spill: 2.7 ms at B=2 H=56/8 S=8192 with 1024
 // keys to either side); alone on its SIMD it moves scores between register files for as
 // long as it multiplies (3.5 ms); and waves of both kinds in one workgroup run their
-// softmax at the same time (2.9 ms).  As it is: 1.8 to 2.0 ms there, 0.9 PFLOP/s of the five
+// softmax at the same time (2.9 ms).  As it is: 1.7 to 1.8 ms there, 1.0 PFLOP/s of the five
 // products, the rest being the tail of the grid (seven heads share a tile's keys, so an
 // item is 238 stages and a place gets four or five of them) and the masked stages.
 //
@@ -1205,8 +1205,8 @@ __global__ void __launch_bounds__(256) window_dkdv_sum_kernel(WindowArgs a) {
 
 // Tiles that hold first keys, and the runs each is cut into: as many as make a run no
 // longer than a window tile's, or than a quarter of what one of the chip's 512 places for
-// workgroups has to do in all, if that is more (it also bounds the partial sums: at most
-// about 1024 runs of 128 KB).  In stages of one query head.  Then, if the tiles' dK and dV
+// workgroups has to do in all, if that is more (it also bounds the partial sums: 1024
+// runs of 128 KB and one more per tile, and fewer than 1024 tiles are cut: 256 MB).  In stages of one query head.  Then, if the tiles' dK and dV
 // fill less than half of the places, all of them may be cut into more runs, of four stages
 // at least: the join costs about four stages, and ten if 512 runs leave partial sums
 // (H=8/1 S=1568, 119 and 26 keys to the sides: 82 us in 26 workgroups, 27 with the join).
@@ -1247,7 +1247,8 @@ size_t window_bwd_bytes(WindowArgs a) {
 }
 
 // Grid of `tiles` work items for each of a batch's `heads` heads (item_of).  Runs are as long
-// as they can be, up to 64 tiles, with a multiple of 8 to a sequence: neighbours share more of
+// as they can be, up to 64 tiles, with a multiple of 8 to a sequence where the number of a
+// head's tiles allows it: neighbours share more of
 // what they read in an XCD's L2, and every XCD gets as many (dK and dV, against runs of a
 // 128th of all tiles: 2.29 -> 2.01 ms at B=2 H=56/8 S=8192, 122 -> 111 us at H=14 S=4104;
 // forward, runs of 16 tiles against 64: 10.0 -> 9.2 ms at H=56 S=42120).  Where sequences may
