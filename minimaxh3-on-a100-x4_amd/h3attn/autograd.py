@@ -2,7 +2,9 @@
 
 Each is a torch.autograd.Function over the forward and backward entry points: inputs are
 saved as they are given, statistics in fp32, and nothing is recomputed but what the
-backward kernels recompute themselves.  Gradients that are not asked for are not returned.
+backward kernels recompute themselves.  Gradients that are not asked for are not returned;
+the attention's and the prologue's backward passes take their full time all the same (the
+layer norm's leaves its weights' gradients out).
 
 A backward pass is captured into a HIP graph as torch's own are: on leaves that no eager
 graph still alive holds (torch.autograd.grad on fresh leaves, or after such graphs are
